@@ -1,0 +1,996 @@
+// Softmax cross entropy of a linear vocabulary head without its logits, and its gradient, on the 5th-generation
+// tensor cores (sm_100a).
+//
+//   z[i][v] = sum_k h[i][k] w[v][k] + b[v],   loss[i] = log sum_v exp z[i][v] - z[i][label_i]
+//   g[i][v] = c_i (exp(z[i][v] - lse_i) - [v = label_i]),   dh = g w,   dw = g^T h,   db[v] = sum_i g[i][v]
+//
+// with c_i the weight of row i in the reduced loss (0 for an ignored row).
+//
+// Loss: one tensor-core product whose epilogue reduces each 128-column slice of a row to (maximum, sum of
+// exponentials) in 32 bits while the accumulator is in tensor memory; the logits never reach memory.
+// xent_finish_kernel joins a row's slices. Bound by the product: 2 rows vocab hidden operations.
+// Gradient: rows go through in chunks (all of them in one, unless 16 bits x rows x vocab pass the chunk limit). The same
+// product also leaves e = exp(z - slice maximum), rounded to the operands' 16-bit type, in the workspace;
+// once lse is known xent_rescale_kernel turns e into g in place (one read and one write of 16 bits per
+// logit: 4 bytes against 6 hidden operations), and two more products read g: dh directly, dw with both
+// operands taken along their non-contiguous direction (MN-major tiles), so nothing is transposed in memory.
+// Keeping e for a chunk of rows costs its two passes; recomputing the logits instead would cost a
+// fourth product of the size of the other three.
+// g is rounded to 16 bits twice (e, then g: at most half a step each), sums are 32-bit throughout. For fp16 both
+// carry a factor 2^15 (their values lie in [-1, 1], most of them far below fp16's smallest normal number).
+//
+// The product kernel is persistent, a CTA pair per 256 x 256 tile (cta_group::2): warp 0 feeds a six-stage ring
+// by TMA, one thread of the leader issues tcgen05.mma into one of two 256-column accumulators, eight warps
+// empty the other one. All waits are bounded; a wait that gives up sets the error flag and every role leaves.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "sm100.cuh"
+
+namespace evox {
+namespace {
+
+constexpr int TM = 256, TN = 256, BK = 64, STAGES = 6;  // one tile of a CTA pair; each CTA holds half of both operands
+constexpr int kThreads = 64 + 256;
+constexpr uint32_t kOperandBytes = 128 * BK * 2;
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kOffBars = STAGES * kStageBytes;
+constexpr uint32_t kSmemBytes = kOffBars + 256;
+constexpr int kSlice = 128;  // columns that one (maximum, sum) covers
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum { kLoss = 0, kProb = 1, kOut = 2 };
+
+struct ProductArgs {
+  long long M, N;
+  int k_blocks;            // of BK
+  int splits;              // the reduction is divided among this many work items per tile
+  int tiles_m, tiles_n;
+  int m_fast, group;       // tiles run through `group` of the one direction, then all of the other
+  uint32_t idesc;
+  int* error_flag;
+  // kLoss, kProb
+  const float* bias;       // [N] or null
+  const long long* labels; // [M]
+  float2* stats;           // [slices][ld_stats]: (maximum, sum of exponentials)
+  long long ld_stats;
+  float* label_logit;      // [M]
+  void* e;                 // [M][ld_e], kProb
+  long long ld_e;
+  // kOut
+  void* out16;             // [M][ld_out] (final), or null
+  float* out32;            // [splits][M][ld32] partial sums, or the running sum over row chunks, or null
+  long long ld_out, ld32;
+  int vec16;               // rows of out16 start on 16-byte boundaries
+  int add32;               // add what out32 holds before storing (or to out16)
+  const float* scale;      // device scalar
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool FP16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (FP16) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  } else {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+}
+template <bool FP16>
+__device__ __forceinline__ unsigned short pack1(float a) {
+  if constexpr (FP16) return __half_as_ushort(__float2half_rn(a));
+  else return __bfloat16_as_ushort(__float2bfloat16_rn(a));
+}
+template <bool FP16>
+__device__ __forceinline__ float2 unpack2(uint32_t p) {
+  if constexpr (FP16) return __half22float2(*reinterpret_cast<const __half2*>(&p));
+  else return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+template <bool FP16>
+constexpr float kProbScale = FP16 ? 32768.0f : 1.0f;
+
+// Operand descriptor of an MN-major tile: 64 elements of the row direction are contiguous (128 bytes, swizzled), one
+// such line per reduction index; 8 lines make 1,024 bytes, the next 64 row elements start 64 lines further.
+__device__ __forceinline__ unsigned long long umma_desc_mn(uint32_t smem_addr) {
+  return umma_desc(smem_addr) | ((unsigned long long)((64u * 128u) >> 4) << 16);
+}
+
+struct Tile {
+  int m, n, split;
+};
+__device__ __forceinline__ Tile tile_of(const ProductArgs& a, long long work) {
+  const long long tiles = (long long)a.tiles_m * a.tiles_n;
+  Tile t;
+  t.split = (int)(work / tiles);
+  const long long r = work - (long long)t.split * tiles;
+  const int fast = a.m_fast ? a.tiles_m : a.tiles_n, slow = a.m_fast ? a.tiles_n : a.tiles_m;
+  const int first = (int)(r / ((long long)a.group * slow)) * a.group;
+  const int width = min(a.group, fast - first);
+  const long long q = r - (long long)first * slow;
+  const int s = (int)(q / width), f = first + (int)(q - (long long)s * width);
+  t.m = a.m_fast ? f : s;
+  t.n = a.m_fast ? s : f;
+  return t;
+}
+
+// D = A B^T over the reduction index; A_MN / B_MN: that operand is contiguous along its own rows instead.
+template <int MODE, bool A_MN, bool B_MN, bool FP16>
+__global__ void __launch_bounds__(kThreads, 1)
+    xent_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = smem_u32(smem_raw);
+  if ((smem_base & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned window: refuse to run otherwise
+    if (threadIdx.x == 0) atomicCAS(a.error_flag, 0, 5);
+    return;
+  }
+  const uint32_t bars = smem_base + kOffBars;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto tfull_bar = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+  auto tempty_bar = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + kOffBars + 8 * (2 * STAGES + 4));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_rank();
+  const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
+  const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  auto kb_range = [&](int split, int& kb0, int& kb1) {
+    kb0 = (int)((long long)split * a.k_blocks / a.splits);
+    kb1 = (int)((long long)(split + 1) * a.k_blocks / a.splits);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * 256);  // the leader's collects both epilogues
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers exist before anything is sent to them
+  fence_after_sync();
+  const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+
+  if (warp == 0) {
+    // ------------------------------- TMA producer ------------------------------------------
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, issued = 0;
+      bool ok = true;
+      const uint32_t leader_full0 = map_to_cta(full_bar(0), 0u);
+      for (long long work = first; work < n_work && ok; work += step) {
+        const Tile t = tile_of(a, work);
+        const int m0 = t.m * TM + (int)cta_rank * 128, n0 = t.n * TN + (int)cta_rank * 128;
+        int kb0, kb1;
+        kb_range(t.split, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) {
+            ok = false;
+            break;
+          }
+          if (cta_rank == 0) mbar_expect_tx(full_bar(s), 2 * kStageBytes);
+          const uint32_t fb = leader_full0 + 8u * s, sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
+          const int k0 = kb * BK;
+          if constexpr (A_MN) {
+            tma_load_2d_pair(sa, &map_a, fb, m0, k0);
+            tma_load_2d_pair(sa + kOperandBytes / 2, &map_a, fb, m0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sa, &map_a, fb, k0, m0);
+          }
+          if constexpr (B_MN) {
+            tma_load_2d_pair(sb, &map_b, fb, n0, k0);
+            tma_load_2d_pair(sb + kOperandBytes / 2, &map_b, fb, n0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sb, &map_b, fb, k0, n0);
+          }
+          issued |= 1u << s;
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // the leader's releases of this CTA's stages arrive asynchronously: see the last one of every stage land
+      // before this CTA may leave
+      for (int q = 0; q < STAGES && ok; ++q) {
+        if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) ok = false;
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if (!ok) {
+        // drain: the last copy issued into each stage must land before shared memory is released; the follower's
+        // copies report to the leader, so it cannot see them
+        for (int q = 0; q < STAGES && cta_rank == 0; ++q) {
+          if (!(issued & (1u << q))) continue;
+          const uint32_t last = (q < s) ? ph : (ph ^ 1u);
+          const unsigned long long t0 = global_timer_ns();
+          while (!mbar_try(full_bar(q), last) && !mbar_try(full_bar(q), last ^ 1u)) {
+            if (global_timer_ns() - t0 > kWaitLimitNs) break;
+          }
+        }
+        // copies and products that nothing here can observe: give them a millisecond, far beyond their latency
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer --------------------------------------------
+    if (lane == 0 && cta_rank == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      long long it = 0;
+      bool ok = true;
+      for (long long work = first; work < n_work && ok; work += step, ++it) {
+        const Tile t = tile_of(a, work);
+        int kb0, kb1;
+        kb_range(t.split, kb0, kb1);
+        const int buf = (int)(it & 1);
+        if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) break;
+        fence_after_sync();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(buf * TN);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          const uint32_t sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            // 16 reduction indices further: 32 bytes along a K-major line, 16 lines of an MN-major tile
+            const unsigned long long da = A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32);
+            const unsigned long long db = B_MN ? umma_desc_mn(sb + k * 2048) : umma_desc(sb + k * 32);
+            umma_f16_pair(d_tmem, da, db, a.idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit_pair(empty_bar(s));  // stage reusable in both CTAs once these products have read it
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) umma_commit_pair(tfull_bar(buf));  // accumulator complete
+      }
+    }
+  } else {
+    // ------------------------------- epilogue (256 threads) --------------------------------
+    const int quarter = warp & 3;          // TMEM lanes this warp may read
+    const int half = (warp - 2) >> 2;      // which 128 of the tile's 256 columns this warp handles
+    const uint32_t leader_tempty0 = map_to_cta(tempty_bar(0), 0u);
+    long long it = 0;
+    for (long long work = first; work < n_work; work += step, ++it) {
+      const Tile t = tile_of(a, work);
+      const int buf = (int)(it & 1);
+      const long long row = (long long)t.m * TM + cta_rank * 128 + quarter * 32 + lane;
+      const long long col0 = (long long)t.n * TN + half * kSlice;
+      const bool live = row < a.M;
+      const int width = (int)max(0ll, min((long long)kSlice, a.N - col0));  // columns of this slice that exist
+      const bool ready = mbar_wait(tfull_bar(buf), (uint32_t)((it >> 1) & 1), a.error_flag, 4);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      fence_after_sync();
+      const uint32_t taddr = tmem_base + (uint32_t)(buf * TN + half * kSlice) + ((uint32_t)(quarter * 32) << 16);
+      if constexpr (MODE == kOut) {
+        const float scale = a.scale ? __ldg(a.scale) : 1.0f;
+        float* o32 = a.out32 ? a.out32 + ((long long)t.split * a.M + row) * a.ld32 + col0 : nullptr;
+        unsigned short* o16 = a.out16 ? reinterpret_cast<unsigned short*>(a.out16) + row * a.ld_out + col0 : nullptr;
+#pragma unroll
+        for (int c = 0; c < kSlice; c += 32) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld32(taddr + c, v);
+          tmem_ld_wait();
+          if (live && o32) {  // rows of out32 hold a multiple of four columns
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              if (c + j < width) {
+                float4 r = make_float4(__uint_as_float(v[j]) * scale, __uint_as_float(v[j + 1]) * scale,
+                                       __uint_as_float(v[j + 2]) * scale, __uint_as_float(v[j + 3]) * scale);
+                if (a.add32) {
+                  const float4 b = *reinterpret_cast<const float4*>(o32 + c + j);
+                  r.x += b.x; r.y += b.y; r.z += b.z; r.w += b.w;
+                }
+                if (!o16) *reinterpret_cast<float4*>(o32 + c + j) = r;
+                v[j] = __float_as_uint(r.x);
+                v[j + 1] = __float_as_uint(r.y);
+                v[j + 2] = __float_as_uint(r.z);
+                v[j + 3] = __float_as_uint(r.w);
+              }
+            }
+          }
+          if (live && o16) {
+            const float s16 = o32 ? 1.0f : scale;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              if (a.vec16 && c + j + 8 <= width) {
+                uint4 p;
+                p.x = pack2<FP16>(__uint_as_float(v[j]) * s16, __uint_as_float(v[j + 1]) * s16);
+                p.y = pack2<FP16>(__uint_as_float(v[j + 2]) * s16, __uint_as_float(v[j + 3]) * s16);
+                p.z = pack2<FP16>(__uint_as_float(v[j + 4]) * s16, __uint_as_float(v[j + 5]) * s16);
+                p.w = pack2<FP16>(__uint_as_float(v[j + 6]) * s16, __uint_as_float(v[j + 7]) * s16);
+                *reinterpret_cast<uint4*>(o16 + c + j) = p;
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (c + j + i < width) o16[c + j + i] = pack1<FP16>(__uint_as_float(v[j + i]) * s16);
+              }
+            }
+          }
+        }
+      } else {
+        const long long label = live ? __ldg(a.labels + row) - col0 : -1;  // within this slice?
+        // one 32-column piece of the row's logits; columns past the vocabulary become -inf
+        auto logits = [&](int c, float (&z)[32]) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld32(taddr + c, v);
+          tmem_ld_wait();
+          if (c + 32 <= width) {
+            if (a.bias) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]) + __ldg(a.bias + col0 + c + j);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              z[j] = c + j < width ? __uint_as_float(v[j]) + (a.bias ? __ldg(a.bias + col0 + c + j) : 0.f) : -INFINITY;
+          }
+        };
+        auto keep_label = [&](int c, const float (&z)[32]) {
+          if (__any_sync(0xffffffffu, label >= c && label < c + 32)) {
+            float at = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) at = (label == c + j) ? z[j] : at;
+            if (label >= c && label < c + 32 && label < width) a.label_logit[row] = at;
+          }
+        };
+        float m = -INFINITY, sum = 0.f;
+        if constexpr (MODE == kLoss) {
+#pragma unroll 1
+          for (int c = 0; c < kSlice; c += 32) {
+            float z[32];
+            logits(c, z);
+            float top = z[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
+            top = fmaxf(top, m);
+            const float base = top == -INFINITY ? 0.f : top * kLog2e;
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) part += exp2_approx(fmaf(z[j], kLog2e, -base));
+            sum = fmaf(sum, exp2_approx(fmaf(m, kLog2e, -base)), part);
+            m = top;
+            keep_label(c, z);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kSlice; c += 32) {
+            float z[32];
+            logits(c, z);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) m = fmaxf(m, z[j]);
+            keep_label(c, z);
+          }
+          const float base = m == -INFINITY ? 0.f : m * kLog2e;
+          unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
+#pragma unroll 1
+          for (int c = 0; c < kSlice; c += 32) {
+            float z[32];
+            logits(c, z);
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              z[j] = exp2_approx(fmaf(z[j], kLog2e, -base));
+              part += z[j];
+            }
+            sum += part;
+            if (live && col0 + c < a.ld_e) {  // rows of e hold a multiple of 64 columns
+              constexpr float s = kProbScale<FP16>;
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                uint4 p;
+                p.x = pack2<FP16>(z[j] * s, z[j + 1] * s);
+                p.y = pack2<FP16>(z[j + 2] * s, z[j + 3] * s);
+                p.z = pack2<FP16>(z[j + 4] * s, z[j + 5] * s);
+                p.w = pack2<FP16>(z[j + 6] * s, z[j + 7] * s);
+                *reinterpret_cast<uint4*>(e + c + j) = p;
+              }
+            }
+          }
+        }
+        if (live && width > 0) a.stats[(long long)(t.n * 2 + half) * a.ld_stats + row] = make_float2(m, sum);
+      }
+      fence_before_sync();
+      mbar_arrive_cluster(leader_tempty0 + 8u * buf);  // this thread no longer reads the accumulator
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  // the pair leaves together: until here the peer may still arrive on this CTA's barriers, and the leader's
+  // products read this CTA's shared memory
+  cluster_sync_all();
+  if (warp == 1) {
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+  }
+}
+
+// What a row counts for. valid: its label is not ignore_index. `scalars`: [0] scale of the gradient (its weights are
+// stored as fractions of the largest one, so that any upstream gradient fits the 16-bit type), [1] its inverse,
+// [2] factor of the summed loss. One block: a fixed order, and the counts are whole numbers.
+__global__ void __launch_bounds__(1024)
+    xent_weights_kernel(const long long* __restrict__ labels, long long ignore_index, long long rows, int reduction,
+                        const float* __restrict__ grad_loss, float prob_scale, float* __restrict__ scalars) {
+  __shared__ unsigned long long count_part[32];
+  __shared__ float max_part[32];
+  unsigned long long count = 0;
+  float top = 0.f;
+  for (long long i = threadIdx.x; i < rows; i += 1024) {
+    const bool valid = labels[i] != ignore_index;
+    count += valid;
+    if (reduction == EVOX_REDUCE_NONE && grad_loss && valid) {
+      const float g = fabsf(grad_loss[i]);
+      if (g <= 3.0e38f) top = fmaxf(top, g);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if ((threadIdx.x & 31) == 0) {
+    count_part[threadIdx.x >> 5] = count;
+    max_part[threadIdx.x >> 5] = top;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) {
+      count += count_part[w];
+      top = fmaxf(top, max_part[w]);
+    }
+    const float per_row = reduction == EVOX_REDUCE_MEAN ? 1.0f / (float)count : 1.0f;  // no valid row: the mean is 0 / 0
+    float scale;
+    if (reduction == EVOX_REDUCE_NONE)
+      scale = grad_loss ? (top > 1.0e-36f ? top : 1.0f) : 1.0f;
+    else
+      scale = count == 0 ? 0.f : per_row * (grad_loss ? grad_loss[0] : 1.0f);
+    scalars[0] = scale / prob_scale;
+    scalars[1] = 1.0f / scale;
+    scalars[2] = per_row;
+  }
+}
+
+// lse[i] and loss[i] from the slices' (maximum, sum): lanes are rows, warps share the slices. A label outside the
+// vocabulary that is not ignore_index gives NaN (and NaN gradients): loud, and nothing is read out of bounds.
+__global__ void __launch_bounds__(1024)
+    xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
+                       const long long* __restrict__ labels, long long ignore_index, long long rows, long long vocab,
+                       float* __restrict__ lse, float* __restrict__ loss) {
+  __shared__ float sm[32][33], ss[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows) {
+    for (int j = warp; j < slices; j += 32) {
+      const float2 p = __ldg(stats + (long long)j * ld_stats + row);
+      const float top = fmaxf(m, p.x);
+      const float base = top == -INFINITY ? 0.f : top * kLog2e;
+      s = s * exp2_approx(fmaf(m, kLog2e, -base)) + p.y * exp2_approx(fmaf(p.x, kLog2e, -base));
+      m = top;
+    }
+  }
+  sm[warp][lane] = m;
+  ss[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && row < rows) {
+    for (int w = 1; w < 32; ++w) m = fmaxf(m, sm[w][lane]);
+    const float base = m == -INFINITY ? 0.f : m;
+    s = 0.f;
+    for (int w = 0; w < 32; ++w) s += ss[w][lane] * expf(sm[w][lane] - base);
+    float l = m + logf(s);
+    const long long y = labels[row];
+    if (y != ignore_index && (y < 0 || y >= vocab)) l = NAN;
+    if (lse) lse[row] = l;
+    loss[row] = y == ignore_index ? 0.f : (l != l ? l : l - label_logit[row]);
+  }
+}
+
+// e -> g in place (see the head of the file), 128 rows x 1,024 columns per block, eight columns per thread; column sums
+// of the block's rows for the bias gradient. The blocks of the last grid row copy the hidden states for the weight
+// gradient, with zeros where the label is ignored: 0 x inf in a padded row must not reach dw.
+template <bool FP16>
+__global__ void __launch_bounds__(256)
+    xent_rescale_kernel(unsigned short* __restrict__ e, long long ld_e, const float2* __restrict__ stats, long long ld_stats, int slices,
+                        const float* __restrict__ lse, const long long* __restrict__ labels, long long ignore_index,
+                        const float* __restrict__ grad_loss, int per_row, const float* __restrict__ scalars, long long rows,
+                        long long vocab, float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h,
+                        long long hidden, unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks) {
+  const long long row0 = (long long)blockIdx.x * 128;
+  const int n_rows = (int)min(128ll, rows - row0);
+  if ((int)blockIdx.y >= column_blocks) {
+    for (long long i = threadIdx.x; i < n_rows * (ld_h_out / 8); i += 256) {
+      const long long r = i / (ld_h_out / 8), c = (i - r * (ld_h_out / 8)) * 8;
+      uint4 p = make_uint4(0u, 0u, 0u, 0u);
+      if (labels[row0 + r] != ignore_index) {
+        const unsigned short* src = h + (row0 + r) * ld_h + c;
+        if (c + 8 <= hidden) {
+          p = *reinterpret_cast<const uint4*>(src);
+        } else {  // the row may end here
+          unsigned short* q = reinterpret_cast<unsigned short*>(&p);
+          for (int j = 0; j < 8; ++j)
+            if (c + j < hidden) q[j] = src[j];
+        }
+      }
+      *reinterpret_cast<uint4*>(h_out + (row0 + r) * ld_h_out + c) = p;
+    }
+    return;
+  }
+  __shared__ float factor[128][8];
+  __shared__ float weight[128];
+  __shared__ int target[128];
+  __shared__ float sums[128][8];
+  const int tid = threadIdx.x;
+  const long long col_base = (long long)blockIdx.y * 1024;
+  const float inverse = scalars[1];
+  if (tid < n_rows) {
+    const long long y = labels[row0 + tid];
+    const bool valid = y != ignore_index;
+    weight[tid] = valid ? (per_row && grad_loss ? grad_loss[row0 + tid] * inverse : 1.0f) : 0.f;
+    const long long d = y - col_base;
+    target[tid] = valid && d >= 0 && d < 1024 ? (int)d : -1;
+  }
+  __syncthreads();
+  for (int i = tid; i < 8 * 128; i += 256) {
+    const int s = i >> 7, r = i & 127;
+    const long long slice = col_base / kSlice + s;
+    float f = 0.f;
+    if (r < n_rows && slice < slices) {
+      const float m = stats[slice * ld_stats + row0 + r].x;
+      // w = 0 (an ignored row) stays 0 whatever the row holds: 0 x NaN is not formed
+      f = weight[r] == 0.f ? 0.f : exp2_approx((m - lse[row0 + r]) * kLog2e) * weight[r];
+    }
+    factor[r][s] = f;
+  }
+  __syncthreads();
+  const int group = tid & 127, part = tid >> 7;  // eight columns; which half of the rows
+  const long long col = col_base + group * 8;
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  if (col < ld_e) {
+#pragma unroll 4
+    for (int r = part; r < n_rows; r += 2) {
+      uint4* at = reinterpret_cast<uint4*>(e + (row0 + r) * ld_e + col);
+      const float f = factor[r][group >> 4];
+      uint4 p = make_uint4(0u, 0u, 0u, 0u);
+      if (weight[r] != 0.f) {
+        p = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+        const int t = target[r] - group * 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 x = unpack2<FP16>(w[j]);
+          x.x *= f;
+          x.y *= f;
+          if (t == 2 * j) x.x = fmaf(-kProbScale<FP16>, weight[r], x.x);
+          if (t == 2 * j + 1) x.y = fmaf(-kProbScale<FP16>, weight[r], x.y);
+          acc[2 * j] += x.x;
+          acc[2 * j + 1] += x.y;
+          w[j] = pack2<FP16>(x.x, x.y);
+        }
+      }
+      *at = p;
+    }
+  }
+  if (bias_partial) {
+    if (part == 1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[group][j] = acc[j];
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < vocab) bias_partial[(long long)blockIdx.x * vocab + col + j] = acc[j] + sums[group][j];
+    }
+  }
+}
+
+// db[v] (+)= scale * sum over the row blocks, in their order.
+__global__ void __launch_bounds__(256)
+    xent_bias_kernel(const float* __restrict__ partial, int blocks, long long vocab, const float* __restrict__ scalars, int add,
+                     float* __restrict__ db) {
+  const long long v = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (v >= vocab) return;
+  float s = 0.f;
+  for (int b = 0; b < blocks; ++b) s += partial[(long long)b * vocab + v];
+  s *= scalars[0];
+  db[v] = add ? db[v] + s : s;
+}
+
+// out[r][c] = sum over the splits, in their order, of partial[split][r][c] (partials are scaled already).
+template <bool FP16>
+__global__ void __launch_bounds__(256)
+    xent_join_kernel(const float* __restrict__ partial, int splits, long long rows, long long cols, long long ld32,
+                     unsigned short* __restrict__ out, long long ld_out) {
+  const long long quads = (cols + 3) / 4, n = rows * quads;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / quads, c = (i - r * quads) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < splits; ++k) {
+      const float4 p = *reinterpret_cast<const float4*>(partial + ((long long)k * rows + r) * ld32 + c);
+      s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < cols) out[r * ld_out + c + j] = pack1<FP16>(v[j]);
+  }
+}
+
+// Sum of the rows' losses times the reduction's factor: one block, 64-bit sums in a fixed order.
+__global__ void __launch_bounds__(1024)
+    xent_loss_sum_kernel(const float* __restrict__ loss, long long rows, const float* __restrict__ scalars, float* __restrict__ out) {
+  __shared__ double part[32];
+  double s = 0.0;
+  for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) s += part[w];
+    out[0] = (float)(s * (double)scalars[2]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+long long up(long long x, long long m) { return (x + m - 1) / m * m; }
+
+// Map of a 16-bit matrix (`outer` lines of `inner` elements, `ld` apart) with boxes of 64 elements x `box_outer` lines.
+int map_16(CUtensorMap* map, const void* base, long long inner, long long outer, long long ld, int box_outer, bool fp16) {
+  EncodeTiledFn fn;
+  if (int rc = encode_fn(&fn)) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64u, (cuuint32_t)box_outer};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  EVOX_REQUIRE(r == CUDA_SUCCESS, EVOX_ERR_CUDA, "linear_cross_entropy: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return EVOX_OK;
+}
+
+template <int MODE, bool A_MN, bool B_MN, bool FP16>
+int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, ProductArgs& a, cudaStream_t stream) {
+  a.tiles_m = (int)((a.M + TM - 1) / TM);
+  a.tiles_n = (int)((a.N + TN - 1) / TN);
+  const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
+  const int fast = a.m_fast ? a.tiles_m : a.tiles_n;
+  if (a.group > fast) a.group = fast;
+  // fp32 accumulator, both operands of the one 16-bit type, 256 x 256; MN-major operands at bits 15 and 16
+  a.idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) |
+            (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+  const long long slots = sm_count() / 2;
+  const long long pairs = n_work < slots ? n_work : slots;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, A_MN, B_MN, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
+  EVOX_CUDA(cudaLaunchKernelEx(&cfg, xent_product_kernel<MODE, A_MN, B_MN, FP16>, map_a, map_b, a));
+  return EVOX_OK;
+}
+
+// Rows (or columns) of tiles that run together so that their operand, `bytes_per_tile` each, stays in the L2 cache
+// next to what streams past it.
+int resident_group(long long bytes_per_tile) {
+  const long long g = (48ll << 20) / (bytes_per_tile > 0 ? bytes_per_tile : 1);
+  return (int)(g < 1 ? 1 : (g > 1024 ? 1024 : g));
+}
+
+// Work items per tile of a product with few tiles: enough to fill the CTA pairs, at least eight blocks of the
+// reduction each, at most 16.
+int reduction_splits(long long M, long long N, long long K) {
+  const long long tiles = ((M + TM - 1) / TM) * ((N + TN - 1) / TN), slots = sm_count() / 2, kb = (K + BK - 1) / BK;
+  long long s = slots / tiles;
+  if (s > kb / 8) s = kb / 8;
+  if (s > 16) s = 16;
+  return (int)(s < 1 ? 1 : s);
+}
+
+struct Carve {  // 256-byte aligned pieces of the workspace
+  uint8_t* base;
+  size_t used;
+  template <class T>
+  T* take(size_t count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += (count * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+struct Buffers {
+  float* scalars;
+  float2* stats;
+  float* label_logit;
+  float* lse;
+  float* loss;
+  unsigned short* e;
+  unsigned short* h_copy;
+  float* bias_partial;
+  float* partial;  // split products of dh or dw
+  float* dw_sum;   // running dw over the row chunks
+};
+
+size_t layout(Buffers& b, void* base, long long rows, long long hidden, long long vocab, long long chunk, bool grad, bool with_bias) {
+  Carve c{reinterpret_cast<uint8_t*>(base), 0};
+  const long long slices = (vocab + kSlice - 1) / kSlice;
+  b.scalars = c.take<float>(4);
+  b.stats = c.take<float2>((size_t)slices * chunk);
+  b.label_logit = c.take<float>(chunk);
+  b.loss = c.take<float>(rows);
+  if (grad) {
+    b.lse = c.take<float>(chunk);
+    b.e = c.take<unsigned short>((size_t)chunk * up(vocab, 64));
+    b.h_copy = c.take<unsigned short>((size_t)chunk * up(hidden, 8));
+    b.bias_partial = with_bias ? c.take<float>((size_t)((chunk + 127) / 128) * vocab) : nullptr;
+    size_t part = 0;
+    for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
+      const int sh = reduction_splits(r, hidden, vocab), sw = reduction_splits(vocab, hidden, r);
+      if (sh > 1 && part < (size_t)sh * r * up(hidden, 4)) part = (size_t)sh * r * up(hidden, 4);
+      if (sw > 1 && part < (size_t)sw * vocab * up(hidden, 4)) part = (size_t)sw * vocab * up(hidden, 4);
+    }
+    b.partial = part ? c.take<float>(part) : nullptr;
+    b.dw_sum = chunk < rows ? c.take<float>((size_t)vocab * up(hidden, 4)) : nullptr;
+  }
+  return c.used;
+}
+
+int check_operands(const char* what, const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype, const int64_t* labels,
+                   int64_t rows, int64_t hidden, int64_t vocab, int32_t reduction, const float* loss, const void* workspace,
+                   const int32_t* error_flag) {
+  EVOX_REQUIRE(h && w && labels && loss && workspace && error_flag, EVOX_ERR_INVALID, "%s: NULL pointer", what);
+  EVOX_REQUIRE(rows > 0 && hidden > 0 && vocab > 0 && rows < (1ll << 30) && hidden < (1ll << 26) && vocab < (1ll << 26), EVOX_ERR_INVALID,
+               "%s: rows must be in [1, 2^30), hidden and vocab in [1, 2^26), got %lld, %lld, %lld", what, (long long)rows, (long long)hidden, (long long)vocab);
+  EVOX_REQUIRE(dtype == EVOX_DTYPE_BF16 || dtype == EVOX_DTYPE_FP16, EVOX_ERR_INVALID, "%s: operands must be bf16 or fp16", what);
+  EVOX_REQUIRE(reduction == EVOX_REDUCE_NONE || reduction == EVOX_REDUCE_SUM || reduction == EVOX_REDUCE_MEAN, EVOX_ERR_INVALID,
+               "%s: unknown reduction %d", what, reduction);
+  EVOX_REQUIRE(ld_h >= hidden && ld_w >= hidden && ld_h % 8 == 0 && ld_w % 8 == 0, EVOX_ERR_INVALID,
+               "%s: row strides must be multiples of 8 elements and at least hidden", what);
+  EVOX_REQUIRE(aligned16(h) && aligned16(w), EVOX_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
+  EVOX_REQUIRE(((uintptr_t)workspace & 255u) == 0, EVOX_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
+  return EVOX_OK;
+}
+
+struct Head {
+  const void* h;
+  long long ld_h;
+  const void* w;
+  long long ld_w;
+  const float* bias;
+  const long long* labels;
+  long long ignore_index, rows, hidden, vocab;
+  int* error_flag;
+  cudaStream_t stream;
+};
+
+// Logits of `n` rows from `r0` on: (maximum, sum) per slice, the labels' logits, and with MODE == kProb the exponentials.
+template <int MODE, bool FP16>
+int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats) {
+  CUtensorMap map_a, map_b;
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
+  if (int rc = map_16(&map_a, h, x.hidden, n, x.ld_h, 128, FP16)) return rc;
+  if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
+  ProductArgs a = {};
+  a.M = n;
+  a.N = x.vocab;
+  a.k_blocks = (int)((x.hidden + BK - 1) / BK);
+  a.splits = 1;
+  a.m_fast = 1;  // the weight streams past, the hidden states stay in L2
+  a.group = resident_group(2ll * TM * x.hidden);
+  a.error_flag = x.error_flag;
+  a.bias = x.bias;
+  a.labels = x.labels + r0;
+  a.stats = b.stats;
+  a.ld_stats = ld_stats;
+  a.label_logit = b.label_logit;
+  a.e = MODE == kProb ? b.e : nullptr;
+  a.ld_e = up(x.vocab, 64);
+  return launch_product<MODE, false, false, FP16>(map_a, map_b, a, x.stream);
+}
+
+template <bool FP16>
+int finish_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats, float* lse, float* loss) {
+  const int slices = (int)((x.vocab + kSlice - 1) / kSlice);
+  xent_finish_kernel<<<(unsigned)((n + 31) / 32), 1024, 0, x.stream>>>(b.stats, ld_stats, slices, b.label_logit, x.labels + r0,
+                                                                     x.ignore_index, n, x.vocab, lse, loss + r0);
+  EVOX_LAUNCH_CHECK();
+  return EVOX_OK;
+}
+
+// out (M x N, 16 bits, dense) = scale * A B^T with the reduction divided where that fills the machine better.
+// `sum`: running 32-bit sum over row chunks (null: this product is the whole); `first`, `last`: which chunk.
+template <bool A_MN, bool FP16>
+int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long long M, long long N, long long K, int m_fast, int group,
+                     void* out, const float* scale, float* partial, float* sum, bool first, bool last, int* error_flag,
+                     cudaStream_t stream) {
+  ProductArgs a = {};
+  a.M = M;
+  a.N = N;
+  a.k_blocks = (int)((K + BK - 1) / BK);
+  a.splits = sum ? 1 : reduction_splits(M, N, K);
+  a.m_fast = m_fast;
+  a.group = group;
+  a.error_flag = error_flag;
+  a.scale = scale;
+  a.ld_out = N;
+  a.ld32 = up(N, 4);
+  a.vec16 = N % 8 == 0 && aligned16(out);
+  if (sum) {
+    a.out32 = sum;
+    a.add32 = !first;
+    a.out16 = last ? out : nullptr;
+  } else if (a.splits > 1) {
+    a.out32 = partial;
+  } else {
+    a.out16 = out;
+  }
+  if (int rc = launch_product<kOut, A_MN, true, FP16>(map_a, map_b, a, stream)) return rc;
+  if (a.splits > 1) {
+    const long long n = M * ((N + 3) / 4), blocks = (n + 255) / 256, cap = 16ll * sm_count();
+    xent_join_kernel<FP16><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(partial, a.splits, M, N, a.ld32,
+                                                                                    reinterpret_cast<unsigned short*>(out), N);
+    EVOX_LAUNCH_CHECK();
+  }
+  return EVOX_OK;
+}
+
+template <bool FP16>
+int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reduction, const float* grad_loss, void* dh, void* dw, float* db) {
+  const int slices = (int)((x.vocab + kSlice - 1) / kSlice);
+  const long long ld_e = up(x.vocab, 64), ld_copy = up(x.hidden, 8);
+  for (long long r0 = 0; r0 < x.rows; r0 += chunk) {
+    const long long n = x.rows - r0 < chunk ? x.rows - r0 : chunk;
+    const bool first = r0 == 0, last = r0 + n == x.rows;
+    if (int rc = logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
+    if (int rc = finish_pass<FP16>(x, b, r0, n, chunk, b.lse, b.loss)) return rc;
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
+    const int column_blocks = (int)((x.vocab + 1023) / 1024), row_blocks = (int)((n + 127) / 128);
+    xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (dw ? 1 : 0))), 256, 0, x.stream>>>(
+        b.e, ld_e, b.stats, chunk, slices, b.lse, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
+        reduction == EVOX_REDUCE_NONE, b.scalars, n, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, b.h_copy, ld_copy,
+        column_blocks);
+    EVOX_LAUNCH_CHECK();
+    if (db) {
+      xent_bias_kernel<<<(unsigned)((x.vocab + 255) / 256), 256, 0, x.stream>>>(b.bias_partial, row_blocks, x.vocab, b.scalars, !first, db);
+      EVOX_LAUNCH_CHECK();
+    }
+    CUtensorMap map_a, map_b;
+    if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
+      if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 128, FP16)) return rc;
+      if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
+      unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;
+      if (int rc = gradient_product<false, FP16>(map_a, map_b, n, x.hidden, x.vocab, 0, 8, out, b.scalars, b.partial, nullptr, true, true,
+                                                 x.error_flag, x.stream))
+        return rc;
+    }
+    if (dw) {  // g^T (contiguous along vocab) times the hidden states (contiguous along hidden)
+      if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 64, FP16)) return rc;
+      if (int rc = map_16(&map_b, b.h_copy, x.hidden, n, ld_copy, 64, FP16)) return rc;
+      if (int rc = gradient_product<true, FP16>(map_a, map_b, x.vocab, x.hidden, n, 0, resident_group(2ll * TN * n), dw, b.scalars,
+                                                b.partial, b.dw_sum, first, last, x.error_flag, x.stream))
+        return rc;
+    }
+  }
+  return EVOX_OK;
+}
+
+}  // namespace
+}  // namespace evox
+
+using namespace evox;
+
+extern "C" size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
+  if (rows <= 0 || hidden <= 0 || vocab <= 0) return 0;
+  Buffers b = {};
+  return layout(b, nullptr, rows, hidden, vocab, rows, false, false);
+}
+
+extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype, const float* bias,
+                                         const int64_t* labels, int64_t ignore_index, int64_t rows, int64_t hidden, int64_t vocab,
+                                         int32_t reduction, float* loss, void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                                         void* stream) {
+  if (int rc = check_operands("linear_cross_entropy", h, ld_h, w, ld_w, dtype, labels, rows, hidden, vocab, reduction, loss, workspace, error_flag))
+    return rc;
+  Buffers b = {};
+  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, rows, false, false), EVOX_ERR_WORKSPACE,
+               "linear_cross_entropy: workspace too small");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
+  if (int rc = dtype == EVOX_DTYPE_FP16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
+  float* per_row = reduction == EVOX_REDUCE_NONE ? loss : b.loss;
+  if (int rc = finish_pass<false>(x, b, 0, rows, rows, nullptr, per_row)) return rc;
+  if (reduction != EVOX_REDUCE_NONE) {
+    xent_weights_kernel<<<1, 1024, 0, s>>>(x.labels, ignore_index, rows, reduction, nullptr, 1.0f, b.scalars);
+    EVOX_LAUNCH_CHECK();
+    xent_loss_sum_kernel<<<1, 1024, 0, s>>>(b.loss, rows, b.scalars, loss);
+    EVOX_LAUNCH_CHECK();
+  }
+  return EVOX_OK;
+}
+
+extern "C" int64_t evox_linear_cross_entropy_chunk_rows(int64_t rows, int64_t vocab) {
+  if (rows <= 0 || vocab <= 0) return 0;
+  // 2 GiB of exponentials at most (about 1 % of the memory), in whole tiles of rows
+  const int64_t fit = (2ll << 30) / (up(vocab, 64) * 2) / TM * TM;
+  const int64_t chunk = fit < TM ? TM : fit;
+  return chunk < rows ? chunk : rows;
+}
+
+extern "C" size_t evox_linear_cross_entropy_grad_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab, int64_t chunk_rows,
+                                                                 int32_t with_bias) {
+  if (rows <= 0 || hidden <= 0 || vocab <= 0 || chunk_rows <= 0) return 0;
+  Buffers b = {};
+  return layout(b, nullptr, rows, hidden, vocab, chunk_rows < rows ? chunk_rows : rows, true, with_bias != 0);
+}
+
+extern "C" int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype, const float* bias,
+                                              const int64_t* labels, int64_t ignore_index, int64_t rows, int64_t hidden, int64_t vocab,
+                                              int32_t reduction, const float* grad_loss, int64_t chunk_rows, float* loss, void* dh, void* dw,
+                                              float* dbias, void* workspace, size_t workspace_bytes, int32_t* error_flag, void* stream) {
+  if (int rc = check_operands("linear_cross_entropy_grad", h, ld_h, w, ld_w, dtype, labels, rows, hidden, vocab, reduction, loss, workspace, error_flag))
+    return rc;
+  EVOX_REQUIRE(chunk_rows > 0, EVOX_ERR_INVALID, "linear_cross_entropy_grad: chunk_rows must be positive");
+  const long long chunk = chunk_rows < rows ? chunk_rows : rows;
+  Buffers b = {};
+  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, chunk, true, dbias != nullptr), EVOX_ERR_WORKSPACE,
+               "linear_cross_entropy_grad: workspace too small");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
+  const bool fp16 = dtype == EVOX_DTYPE_FP16;
+  xent_weights_kernel<<<1, 1024, 0, s>>>(x.labels, ignore_index, rows, reduction, grad_loss, fp16 ? kProbScale<true> : kProbScale<false>, b.scalars);
+  EVOX_LAUNCH_CHECK();
+  if (reduction == EVOX_REDUCE_NONE) b.loss = loss;
+  if (int rc = fp16 ? gradient_pass<true>(x, b, chunk, reduction, grad_loss, dh, dw, dbias)
+                    : gradient_pass<false>(x, b, chunk, reduction, grad_loss, dh, dw, dbias))
+    return rc;
+  if (reduction != EVOX_REDUCE_NONE) {
+    xent_loss_sum_kernel<<<1, 1024, 0, s>>>(b.loss, rows, b.scalars, loss);
+    EVOX_LAUNCH_CHECK();
+  }
+  return EVOX_OK;
+}

@@ -1,0 +1,179 @@
+"""Softmax cross entropy of a linear vocabulary head, without its logits, on the tensor cores.
+
+`linear_cross_entropy` is `F.cross_entropy(F.linear(h, weight, bias), labels)` for 16-bit operands: the product's
+epilogue reduces every row to its log-sum-exp, so the (rows, vocab) logits never exist. It is differentiable;
+`linear_cross_entropy_grad` returns loss and gradients in one call, without autograd. The same loss for a
+virtual-LoRA population is `lora_kernels.lora_layer_cross_entropy`.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import _cabi
+from .lora_kernels import _pending_flags
+
+__all__ = ["linear_cross_entropy", "linear_cross_entropy_grad"]
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _operand(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`x` (rows, hidden) with rows that start on 16-byte boundaries, and its row stride; a view is used as it is
+    where it can be, anything else is copied."""
+    rows, hidden = x.shape
+    stride = x.stride(0) if rows > 1 else (hidden + 7) // 8 * 8
+    if x.stride(1) == 1 and stride >= hidden and stride % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, stride
+    pad = -hidden % 8
+    x = F.pad(x, (0, pad)) if pad else x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone()
+    return x, hidden + pad
+
+
+def _arguments(h, weight, labels, bias, reduction):
+    """Checked and flattened arguments: (h, weight, labels, bias fp32, leading shape)."""
+    err = _cabi.EvoxKernelError
+    if reduction not in _REDUCTIONS:
+        raise err(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if h.dtype not in _DTYPES or weight.dtype != h.dtype:
+        raise err(f"hidden states and weight must both be bfloat16 or both float16, got {h.dtype} and {weight.dtype}")
+    if weight.ndim != 2 or h.ndim < 1 or h.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise err(f"shape mismatch: hidden states {tuple(h.shape)}, weight {tuple(weight.shape)}")
+    if labels.dtype != torch.int64 or labels.shape != h.shape[:-1]:
+        raise err(f"labels must be int64 of shape {tuple(h.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
+    if bias is not None and (bias.shape != weight.shape[:1] or not bias.is_floating_point()):
+        raise err(f"bias must be floating point of shape ({weight.shape[0]},), got {bias.dtype} {tuple(bias.shape)}")
+    for name, t in (("hidden states", h), ("weight", weight), ("labels", labels), ("bias", bias)):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise err(f"{name} must live on a CUDA device (evox_b200 has no CPU path), got {t.device}")
+        if t.device != h.device:
+            raise err(f"{name} lives on {t.device}, hidden states on {h.device}")
+    return (h.reshape(-1, h.shape[-1]), weight, labels.reshape(-1).contiguous(),
+            None if bias is None else bias.to(torch.float32).contiguous(), tuple(h.shape[:-1]))
+
+
+def _pointer(x: torch.Tensor, name: str) -> int:
+    _cabi.ptr(x[:1, :1] if x.ndim == 2 else x, None, name)  # device checks; the strides were looked at already
+    return x.data_ptr()
+
+
+def _flag(what: str, dev: torch.device) -> torch.Tensor:
+    err = torch.empty(1, dtype=torch.int32, device=dev)
+    if not torch.cuda.is_current_stream_capturing():  # a captured launch's flag belongs to the graph's replays
+        _pending_flags.append((what, err))
+        del _pending_flags[:-256]
+    return err
+
+
+def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
+    dev = h.device
+    rows, hidden = h.shape
+    vocab = weight.shape[0]
+    if rows == 0:
+        return torch.full(shape if reduction == "none" else (), float("nan") if reduction == "mean" else 0.0, device=dev)
+    (h, ld_h), (weight, ld_w) = _operand(h), _operand(weight)
+    loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
+    lib = _cabi.lib
+    nbytes = lib.evox_linear_cross_entropy_workspace_bytes(rows, hidden, vocab)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    err = _flag("linear_cross_entropy", dev)
+    _cabi.check(lib.evox_linear_cross_entropy(
+        _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
+        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(loss), _cabi.ptr(ws), nbytes, _cabi.ptr(err),
+        _cabi.stream_ptr(dev)))
+    return loss
+
+
+def _loss_and_grad(h, weight, labels, bias, ignore_index, reduction, shape, grad_loss, chunk_rows, wanted):
+    """(loss, dh (rows, hidden), dw, dbias fp32); `wanted`: which of the three gradients are computed."""
+    dev = h.device
+    rows, hidden = h.shape
+    vocab = weight.shape[0]
+    dh = torch.empty(rows, hidden, dtype=h.dtype, device=dev) if wanted[0] else None
+    dw = torch.empty(vocab, hidden, dtype=h.dtype, device=dev) if wanted[1] else None
+    db = torch.empty(vocab, dtype=torch.float32, device=dev) if wanted[2] and bias is not None else None
+    if rows == 0:
+        return _loss(h, weight, labels, bias, ignore_index, reduction, shape), dh, *(None if g is None else g.zero_() for g in (dw, db))
+    (h, ld_h), (weight, ld_w) = _operand(h), _operand(weight)
+    loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
+    lib = _cabi.lib
+    chunk = lib.evox_linear_cross_entropy_chunk_rows(rows, vocab) if chunk_rows is None else chunk_rows
+    nbytes = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, hidden, vocab, chunk, db is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    err = _flag("linear_cross_entropy_grad", dev)
+    _cabi.check(lib.evox_linear_cross_entropy_grad(
+        _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
+        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(grad_loss), chunk, _cabi.ptr(loss), _cabi.ptr(dh),
+        _cabi.ptr(dw), _cabi.ptr(db), _cabi.ptr(ws), nbytes, _cabi.ptr(err), _cabi.stream_ptr(dev)))
+    return loss, dh, dw, db
+
+
+def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None, *,
+                              ignore_index: int = -100, reduction: str = "mean", grad_loss: torch.Tensor | None = None,
+                              chunk_rows: int | None = None):
+    """Loss and its gradients in one call: `(loss, dh, dweight, dbias)`, the gradients in their operands' types
+    (`dbias` is None without a bias). Arguments as for `linear_cross_entropy`; `grad_loss` is the upstream gradient
+    (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
+    are held at a time (default: all, up to 2 GiB of them)."""
+    flat, weight, labels, bias_f, shape = _arguments(h.detach(), weight.detach(), labels, None if bias is None else bias.detach(), reduction)
+    if chunk_rows is not None and chunk_rows < 1:
+        raise _cabi.EvoxKernelError(f"chunk_rows must be at least 1, got {chunk_rows}")
+    if grad_loss is not None:
+        want = shape if reduction == "none" else ()
+        if grad_loss.shape != want:
+            raise _cabi.EvoxKernelError(f"grad_loss must have shape {tuple(want)}, got {tuple(grad_loss.shape)}")
+        grad_loss = grad_loss.detach().to(device=flat.device, dtype=torch.float32).contiguous()
+    loss, dh, dw, db = _loss_and_grad(flat, weight, labels, bias_f, ignore_index, reduction, shape, grad_loss, chunk_rows, (True, True, True))
+    return loss, dh.view(h.shape), dw, None if bias is None else db.to(bias.dtype)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """A scalar loss computes its gradients with the forward pass, while the exponentials are there, and scales them by
+    the upstream gradient; per-row losses have one upstream value per row, so theirs are computed in backward."""
+
+    @staticmethod
+    def forward(ctx, h, weight, labels, bias, ignore_index, reduction):
+        flat, w, flat_labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
+        wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        ctx.args = (ignore_index, reduction, shape, h.shape, None if bias is None else bias.dtype)
+        if reduction == "none":
+            ctx.save_for_backward(h, weight, labels, bias)
+            return _loss(flat, w, flat_labels, bias_f, ignore_index, reduction, shape)
+        loss, *grads = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape, None, None, wanted)
+        ctx.save_for_backward(*grads)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        ignore_index, reduction, shape, h_shape, bias_dtype = ctx.args
+        if reduction == "none":
+            h, weight, labels, bias = ctx.saved_tensors
+            flat, w, flat_labels, bias_f, _ = _arguments(h, weight, labels, bias, reduction)
+            wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+            with torch.cuda.device(h.device):
+                _, dh, dw, db = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape,
+                                               grad.to(torch.float32).contiguous(), None, wanted)
+        else:
+            dh, dw, db = (None if g is None else g * grad for g in ctx.saved_tensors)
+        return (None if dh is None else dh.view(h_shape), dw, None, None if db is None else db.to(bias_dtype), None, None)
+
+
+def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None, *,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """`F.cross_entropy(F.linear(h, weight, bias), labels)` in fp32 without the logits.
+
+    `h` (..., hidden) and `weight` (vocab, hidden): both bf16 or both fp16, any sizes and row strides (rows that do not
+    start on 16-byte boundaries are copied); `labels` (...) int64; `bias` (vocab,). Rows labelled `ignore_index`
+    have loss 0, do not count in the mean and get zero gradients, whatever they hold; a label
+    outside the vocabulary gives NaN. `reduction`: "mean", "sum" or "none" (losses shaped like `labels`).
+    Differentiable once in `h`, `weight` and `bias`."""
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearCrossEntropy.apply(h, weight, labels, bias, ignore_index, reduction)
+    return _loss(*_arguments(h, weight, labels, bias, reduction)[:4], ignore_index, reduction, tuple(h.shape[:-1]))

@@ -565,6 +565,45 @@ int evox_nd_rank_static(const float* f, int64_t n, int32_t m, int32_t* rank, int
 int64_t evox_bench_compare_rate_threads(void);
 int evox_bench_compare_rate(const float* in, uint32_t* out, int32_t iterations, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Language-model head: softmax cross entropy of a linear vocabulary layer without its logits, its
+ * gradient, the same loss for a virtual-LoRA population, and clipping by the global gradient norm.
+ * ------------------------------------------------------------------------------------------ */
+#define EVOX_DTYPE_BF16 0
+#define EVOX_DTYPE_FP16 1
+#define EVOX_DTYPE_FP32 2
+#define EVOX_REDUCE_NONE 0 /* one loss per row */
+#define EVOX_REDUCE_SUM 1
+#define EVOX_REDUCE_MEAN 2 /* over the rows whose label is not ignore_index (none: NaN) */
+
+/* loss = log sum_v exp(z_v) - z_label per row, z = h w^T + bias, with h (rows x hidden, row stride
+ * ld_h) and w (vocab x hidden, row stride ld_w) in bf16 or fp16, strides multiples of 8 elements and
+ * 16-byte aligned bases; bias (vocab, fp32) or NULL; fp32 sums. A row whose label is ignore_index has
+ * loss 0; any other label outside [0, vocab) gives NaN. loss: rows values (EVOX_REDUCE_NONE) or one.
+ * The logits are not stored: the workspace holds 8 bytes per row and 128 columns. error_flag: a
+ * device int32, set to 0 by the call and to a status if a bounded device-side wait expired. */
+size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
+int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype,
+                              const float* bias, const int64_t* labels, int64_t ignore_index,
+                              int64_t rows, int64_t hidden, int64_t vocab, int32_t reduction,
+                              float* loss, void* workspace, size_t workspace_bytes,
+                              int32_t* error_flag, void* stream);
+
+/* The loss and its gradient: dh (rows x hidden) and dw (vocab x hidden), dense, in the operands' type,
+ * dbias (vocab, fp32); each may be NULL. grad_loss (device, or NULL for 1): the upstream gradient, one
+ * value, or one per row with EVOX_REDUCE_NONE. Rows are taken chunk_rows at a time, with 16 bits per
+ * logit of one chunk in the workspace; evox_linear_cross_entropy_chunk_rows gives the number that the
+ * Python wrapper uses (at most 2 GiB of them). with_bias: whether dbias will be given. */
+int64_t evox_linear_cross_entropy_chunk_rows(int64_t rows, int64_t vocab);
+size_t evox_linear_cross_entropy_grad_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab,
+                                                      int64_t chunk_rows, int32_t with_bias);
+int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, int64_t ld_w,
+                                   int32_t dtype, const float* bias, const int64_t* labels,
+                                   int64_t ignore_index, int64_t rows, int64_t hidden, int64_t vocab,
+                                   int32_t reduction, const float* grad_loss, int64_t chunk_rows,
+                                   float* loss, void* dh, void* dw, float* dbias, void* workspace,
+                                   size_t workspace_bytes, int32_t* error_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
