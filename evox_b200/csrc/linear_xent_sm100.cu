@@ -11,7 +11,7 @@
 // xent_finish_kernel joins a row's slices. Bound by the product: 2 rows vocab hidden operations.
 // Gradient: rows go through in chunks (all of them in one, unless 16 bits x rows x vocab pass the chunk limit). The same
 // product also leaves e = exp(z - slice maximum), rounded to the operands' 16-bit type, in the workspace;
-// once lse is known xent_rescale_kernel turns e into g in place (one read and one write of 16 bits per
+// once a row's sum is known xent_rescale_kernel turns e into g in place (one read and one write of 16 bits per
 // logit: 4 bytes against 6 hidden operations), and two more products read g: dh directly, dw with both
 // operands taken along their non-contiguous direction (MN-major tiles), so nothing is transposed in memory.
 // Keeping e for a chunk of rows costs its two passes; recomputing the logits instead would cost a
@@ -72,6 +72,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// exp(z - m) of one row's values. The difference is taken before the factor log2(e), not z log2(e) - m log2(e) in one
+// instruction: the maximum's own term is then exactly 1, so that no loss comes out below 0, and a maximum near the end
+// of the range (a mask of the type's lowest value that leaves nothing else) does not overflow.
+__device__ __forceinline__ void exp_from(float (&z)[32], float m) {
+  m = m == -INFINITY ? 0.f : m;  // nothing but -inf: every exponential is 0
+#pragma unroll
+  for (int j = 0; j < 32; ++j) z[j] = exp2_approx((z[j] - m) * kLog2e);
+}
+// Weight of a sum taken at maximum `m` when the maximum becomes `top` >= m.
+__device__ __forceinline__ float rescale_to(float m, float top) { return exp2_approx((m - (top == -INFINITY ? 0.f : top)) * kLog2e); }
 
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -374,13 +385,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
             top = fmaxf(top, m);
-            const float base = top == -INFINITY ? 0.f : top * kLog2e;
+            keep_label(c, z);
+            exp_from(z, top);
             float part = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) part += exp2_approx(fmaf(z[j], kLog2e, -base));
-            sum = fmaf(sum, exp2_approx(fmaf(m, kLog2e, -base)), part);
+            for (int j = 0; j < 32; ++j) part += z[j];
+            sum = fmaf(sum, rescale_to(m, top), part);
             m = top;
-            keep_label(c, z);
           }
         } else {
 #pragma unroll 1
@@ -391,18 +402,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 32; ++j) m = fmaxf(m, z[j]);
             keep_label(c, z);
           }
-          const float base = m == -INFINITY ? 0.f : m * kLog2e;
           unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
 #pragma unroll 1
           for (int c = 0; c < kSlice; c += 32) {
             float z[32];
             logits(c, z);
+            exp_from(z, m);
             float part = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              z[j] = exp2_approx(fmaf(z[j], kLog2e, -base));
-              part += z[j];
-            }
+            for (int j = 0; j < 32; ++j) part += z[j];
             sum += part;
             if (live && col0 + c < a.ld_e) {  // rows of e hold a multiple of 64 columns
               constexpr float s = kProbScale<FP16>;
@@ -480,12 +488,13 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// lse[i] and loss[i] from the slices' (maximum, sum): lanes are rows, warps share the slices. A label outside the
+// loss[i] and norm[i] = (maximum, 1 / sum of exponentials) from the slices' pairs: lanes are rows, warps share the slices.
+// The two stay apart: added into one log-sum-exp, the logarithm would vanish next to a maximum of large size. A label outside the
 // vocabulary that is not ignore_index gives NaN (and NaN gradients): loud, and nothing is read out of bounds.
 __global__ void __launch_bounds__(1024)
     xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
                        const long long* __restrict__ labels, long long ignore_index, long long rows, long long vocab,
-                       float* __restrict__ lse, float* __restrict__ loss) {
+                       float2* __restrict__ norm, float* __restrict__ loss) {
   __shared__ float sm[32][33], ss[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = (long long)blockIdx.x * 32 + lane;
@@ -494,8 +503,7 @@ __global__ void __launch_bounds__(1024)
     for (int j = warp; j < slices; j += 32) {
       const float2 p = __ldg(stats + (long long)j * ld_stats + row);
       const float top = fmaxf(m, p.x);
-      const float base = top == -INFINITY ? 0.f : top * kLog2e;
-      s = s * exp2_approx(fmaf(m, kLog2e, -base)) + p.y * exp2_approx(fmaf(p.x, kLog2e, -base));
+      s = s * rescale_to(m, top) + p.y * rescale_to(p.x, top);
       m = top;
     }
   }
@@ -507,11 +515,10 @@ __global__ void __launch_bounds__(1024)
     const float base = m == -INFINITY ? 0.f : m;
     s = 0.f;
     for (int w = 0; w < 32; ++w) s += ss[w][lane] * expf(sm[w][lane] - base);
-    float l = m + logf(s);
     const long long y = labels[row];
-    if (y != ignore_index && (y < 0 || y >= vocab)) l = NAN;
-    if (lse) lse[row] = l;
-    loss[row] = y == ignore_index ? 0.f : (l != l ? l : l - label_logit[row]);
+    const bool ignored = y == ignore_index, outside = !ignored && (y < 0 || y >= vocab);
+    if (norm) norm[row] = make_float2(m, outside ? NAN : 1.0f / s);
+    loss[row] = ignored ? 0.f : (outside ? NAN : (m - label_logit[row]) + logf(s));
   }
 }
 
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(1024)
 template <bool FP16>
 __global__ void __launch_bounds__(256)
     xent_rescale_kernel(unsigned short* __restrict__ e, long long ld_e, const float2* __restrict__ stats, long long ld_stats, int slices,
-                        const float* __restrict__ lse, const long long* __restrict__ labels, long long ignore_index,
+                        const float2* __restrict__ norm, const long long* __restrict__ labels, long long ignore_index,
                         const float* __restrict__ grad_loss, int per_row, const float* __restrict__ scalars, long long rows,
                         long long vocab, float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h,
                         long long hidden, unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks) {
@@ -567,7 +574,8 @@ __global__ void __launch_bounds__(256)
     if (r < n_rows && slice < slices) {
       const float m = stats[slice * ld_stats + row0 + r].x;
       // w = 0 (an ignored row) stays 0 whatever the row holds: 0 x NaN is not formed
-      f = weight[r] == 0.f ? 0.f : exp2_approx((m - lse[row0 + r]) * kLog2e) * weight[r];
+      const float2 q = norm[row0 + r];
+      f = weight[r] == 0.f ? 0.f : rescale_to(m, q.x) * q.y * weight[r];
     }
     factor[r][s] = f;
   }
@@ -745,7 +753,7 @@ struct Buffers {
   float* scalars;
   float2* stats;
   float* label_logit;
-  float* lse;
+  float2* norm;
   float* loss;
   unsigned short* e;
   unsigned short* h_copy;
@@ -762,7 +770,7 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
   b.label_logit = c.take<float>(chunk);
   b.loss = c.take<float>(rows);
   if (grad) {
-    b.lse = c.take<float>(chunk);
+    b.norm = c.take<float2>(chunk);
     b.e = c.take<unsigned short>((size_t)chunk * up(vocab, 64));
     b.h_copy = c.take<unsigned short>((size_t)chunk * up(hidden, 8));
     b.bias_partial = with_bias ? c.take<float>((size_t)((chunk + 127) / 128) * vocab) : nullptr;
@@ -832,10 +840,10 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
 }
 
 template <bool FP16>
-int finish_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats, float* lse, float* loss) {
+int finish_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats, float2* norm, float* loss) {
   const int slices = (int)((x.vocab + kSlice - 1) / kSlice);
   xent_finish_kernel<<<(unsigned)((n + 31) / 32), 1024, 0, x.stream>>>(b.stats, ld_stats, slices, b.label_logit, x.labels + r0,
-                                                                     x.ignore_index, n, x.vocab, lse, loss + r0);
+                                                                     x.ignore_index, n, x.vocab, norm, loss + r0);
   EVOX_LAUNCH_CHECK();
   return EVOX_OK;
 }
@@ -885,11 +893,11 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     const long long n = x.rows - r0 < chunk ? x.rows - r0 : chunk;
     const bool first = r0 == 0, last = r0 + n == x.rows;
     if (int rc = logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
-    if (int rc = finish_pass<FP16>(x, b, r0, n, chunk, b.lse, b.loss)) return rc;
+    if (int rc = finish_pass<FP16>(x, b, r0, n, chunk, b.norm, b.loss)) return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
     const int column_blocks = (int)((x.vocab + 1023) / 1024), row_blocks = (int)((n + 127) / 128);
     xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (dw ? 1 : 0))), 256, 0, x.stream>>>(
-        b.e, ld_e, b.stats, chunk, slices, b.lse, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
+        b.e, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
         reduction == EVOX_REDUCE_NONE, b.scalars, n, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, b.h_copy, ld_copy,
         column_blocks);
     EVOX_LAUNCH_CHECK();

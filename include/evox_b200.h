@@ -604,6 +604,16 @@ int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, i
                                    float* loss, void* dh, void* dw, float* dbias, void* workspace,
                                    size_t workspace_bytes, int32_t* error_flag, void* stream);
 
+/* norm (one fp32) = 2-norm over all elements of n_tensors dense tensors; with clip != 0 every element is
+ * then multiplied by min(1, max_norm / (norm + 1e-6)) in place (nothing is written when that is 1).
+ * address, numel, dtype (EVOX_DTYPE_*): HOST arrays, read before the call returns; address holds device
+ * addresses, aligned to their element. Tensors may be empty; with clip no two may share memory.
+ * 64-bit sums in a fixed order. */
+size_t evox_grad_norm_workspace_bytes(int32_t n_tensors);
+int evox_clip_grad_norm(const uint64_t* address, const int64_t* numel, const int32_t* dtype,
+                        int32_t n_tensors, float max_norm, int32_t clip, float* norm, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

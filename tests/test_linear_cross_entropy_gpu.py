@@ -8,6 +8,8 @@ Bounds, with u = eps / 2 of the 16-bit type (bf16 2^-8, fp16 2^-11), counted bef
              2 dz + 2^-20 (max |z| + 16) of itself; the products truncate as above over their own length; the
              output is rounded once more (u). fp16: subnormal steps of the scaled g (2^-39) and of the output.
 """
+import math
+
 import pytest
 import torch
 
@@ -237,6 +239,15 @@ def test_masked_vocabulary(cuda):
     assert bool(torch.isinf(linear_cross_entropy(h, w, labels, b, reduction="none")).all())
     b[3] = float("-inf")  # nothing left: 0 / 0
     assert bool(torch.isnan(linear_cross_entropy(h, w, labels, b, reduction="none")).all())
+    # a finite mask over everything leaves 700 equal logits in 32 bits
+    b = torch.full((700,), torch.finfo(torch.float32).min, device=cuda)
+    equal = torch.full((33,), math.log(700.0), dtype=torch.float64, device=cuda)
+    near(linear_cross_entropy(h, w, labels, b, reduction="none"), equal, equal * 2.0**-20, "loss")
+    _, dh, _, db = linear_cross_entropy_grad(h, w, labels, b, reduction="sum")
+    hot = torch.zeros(700, dtype=torch.float64, device=cuda)
+    hot[4] = 33.0
+    near(db, 33.0 / 700 - hot, 33.0 / 700 * 2.0**-7 + hot * 2.0**-7, "db")
+    assert bool(torch.isfinite(dh).all())
 
 
 @gpu
