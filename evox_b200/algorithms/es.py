@@ -11,6 +11,7 @@ import torch.distributed as dist
 
 from .. import _cabi
 from ..core import Algorithm, Mutable, Parameter
+from ..grad_kernels import clip_grad_norm_
 from ..lora_kernels import compute_counter_offsets, lora_gradient_from_seeds
 from ..sharding import group_info, shard_bounds
 
@@ -61,6 +62,22 @@ class _ESBase(Algorithm):
             self.beta1 = Parameter(0.9, dtype=torch.float32, device=device)
             self.beta2 = Parameter(0.999, dtype=torch.float32, device=device)
 
+    def _set_max_grad_norm(self, max_grad_norm: float | None) -> None:
+        assert max_grad_norm is None or max_grad_norm > 0, "max_grad_norm must be greater than 0."
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None  # 0-d tensor: the norm before clipping, of the latest step
+
+    def _clip(self, grads: list[torch.Tensor]) -> None:
+        """Scale the gradient (all its blocks) to at most `max_grad_norm`, in place."""
+        if self.max_grad_norm is None:
+            return
+        if torch.compiler.is_compiling():
+            from .. import ops
+
+            ops.clip_grad_norm_(grads, self.max_grad_norm)
+        else:
+            self.grad_norm = clip_grad_norm_(grads, self.max_grad_norm)
+
     def sigma(self) -> float:
         """Host copy of noise_stdev; refreshed (one sync) when the parameter was modified in place OR rebound to
         another tensor (a fresh tensor's version counter can equal the cached one, so the key also holds the
@@ -90,12 +107,15 @@ class OpenES(_ESBase):
         optimizer: Literal["adam"] | None = None,
         mirrored_sampling: bool = True,
         device: torch.device | None = None,
+        max_grad_norm: float | None = None,
     ):
+        """`max_grad_norm`: the gradient is scaled down to this 2-norm before the update (`grad_norm` keeps the norm it had)."""
         super().__init__()
         device = torch.get_default_device() if device is None else torch.device(device)
         if mirrored_sampling is True:
             assert pop_size % 2 == 0, "When mirrored_sampling is True, pop_size must be a multiple of 2."
         self._common_init(pop_size, center_init, learning_rate, noise_stdev, optimizer, device)
+        self._set_max_grad_norm(max_grad_norm)
         self.dim = center_init.shape[0]
         self.mirrored_sampling = mirrored_sampling
 
@@ -113,7 +133,9 @@ class OpenES(_ESBase):
 
             pop = ops.openes_ask(self.center, noise, self.noise_stdev, self.pop_size)
             fitness = self.evaluate(pop)
-            _update_center(self, ops.openes_gradient(noise, fitness, self.pop_size, self.sigma()))
+            grad = ops.openes_gradient(noise, fitness, self.pop_size, self.sigma())
+            self._clip([grad])
+            _update_center(self, grad)
             return
         pop = torch.empty(self.pop_size, self.dim, dtype=torch.float32, device=dev)
         lib, s = _cabi.lib, _cabi.stream_ptr(dev)
@@ -121,6 +143,7 @@ class OpenES(_ESBase):
         fitness = self.evaluate(pop).to(torch.float32).contiguous()
         grad = torch.empty(self.dim, dtype=torch.float32, device=dev)
         _cabi.check(lib.evox_openes_gradient(_cabi.ptr(noise), _cabi.ptr(fitness), self.pop_size, self.dim, rows, self.sigma(), _cabi.ptr(grad), s))
+        self._clip([grad])
         _update_center(self, grad)
 
 
@@ -368,19 +391,24 @@ class VirtualLoRAES(_ESBase):
         shard: bool = False,
         group=None,
         gradient_passes: int = 3,
+        max_grad_norm: float | None = None,
     ):
         """`gradient_passes`: tensor-core passes of the population gradient (3 = fp32-accurate, the
         default; 1 = bf16 operands; see `lora_gradient_from_seeds`).
         `shard=True` (under an initialised torch.distributed group): every rank keeps the whole
         centre, but the gradient and update of each 2-D block are computed for this rank's rows only
-        and the updated rows are allgathered; seeds are broadcast from rank 0 each generation."""
+        and the updated rows are allgathered; seeds are broadcast from rank 0 each generation.
+        `max_grad_norm`: the gradient over all blocks is scaled down to this 2-norm before the update (`grad_norm`
+        keeps the norm it had); all blocks are then held at once. Not with `shard=True`: no rank has the whole gradient."""
         super().__init__()
         device = torch.get_default_device() if device is None else torch.device(device)
         self.group = group
         self.gradient_passes = gradient_passes
         self.rank, self.world_size = group_info(group) if shard else (0, 1)
         assert lora_rank > 0, "lora_rank must be greater than 0."
+        assert max_grad_norm is None or not shard, "max_grad_norm is not available with shard=True."
         self._common_init(pop_size, center_init, learning_rate, noise_stdev, optimizer, device)
+        self._set_max_grad_norm(max_grad_norm)
         self.param_shapes = [tuple(s) for s in param_shapes]
         self.lora_rank = lora_rank
         self.dim = sum(int(torch.tensor(s).prod()) for s in self.param_shapes)
@@ -399,6 +427,9 @@ class VirtualLoRAES(_ESBase):
             dist.broadcast(self.seeds, src=dist.get_global_rank(self.group, 0) if self.group is not None else 0, group=self.group)
         sigma = self.sigma()
         fitness = self.evaluate((self.center, self.seeds, sigma)).to(torch.float32).contiguous()
+        if self.max_grad_norm is not None:
+            self._clipped_update(fitness, sigma)
+            return
         start = 0
         for shape, offset in zip(self.param_shapes, self.counter_offsets):
             n = int(torch.tensor(shape).prod())
@@ -416,6 +447,15 @@ class VirtualLoRAES(_ESBase):
                 block = self.center[start : start + n]
                 dist.all_gather_into_tensor(block, block[r0 * k : r1 * k].clone(), group=self.group)
             start += n
+
+    def _clipped_update(self, fitness: torch.Tensor, sigma: float) -> None:
+        """The whole gradient, a block after the other in the centre's order, clipped, then one update."""
+        grad = torch.empty_like(self.center)
+        blocks = list(grad.split([int(torch.tensor(s).prod()) for s in self.param_shapes]))
+        for shape, offset, block in zip(self.param_shapes, self.counter_offsets, blocks):
+            lora_gradient_from_seeds(fitness, self.seeds, shape, self.lora_rank, offset, self.pop_size, sigma, out=block, passes=self.gradient_passes)
+        self._clip(blocks)
+        _update_center(self, grad)
 
     def _row_shard(self, shape) -> tuple[int, int] | None:
         """This rank's rows of a 2-D block, or None when the block is not sharded (1-D blocks, a

@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include "sm100.cuh"
+#include "xent.cuh"
 
 namespace evox {
 namespace {
@@ -37,8 +38,6 @@ constexpr uint32_t kOperandBytes = 128 * BK * 2;
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kOffBars = STAGES * kStageBytes;
 constexpr uint32_t kSmemBytes = kOffBars + 256;
-constexpr int kSlice = 128;  // columns that one (maximum, sum) covers
-constexpr float kLog2e = 1.4426950408889634f;
 
 enum { kLoss = 0, kProb = 1, kOut = 2 };
 
@@ -66,23 +65,6 @@ struct ProductArgs {
   int add32;               // add what out32 holds before storing (or to out16)
   const float* scale;      // device scalar
 };
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// exp(z - m) of one row's values. The difference is taken before the factor log2(e), not z log2(e) - m log2(e) in one
-// instruction: the maximum's own term is then exactly 1, so that no loss comes out below 0, and a maximum near the end
-// of the range (a mask of the type's lowest value that leaves nothing else) does not overflow.
-__device__ __forceinline__ void exp_from(float (&z)[32], float m) {
-  m = m == -INFINITY ? 0.f : m;  // nothing but -inf: every exponential is 0
-#pragma unroll
-  for (int j = 0; j < 32; ++j) z[j] = exp2_approx((z[j] - m) * kLog2e);
-}
-// Weight of a sum taken at maximum `m` when the maximum becomes `top` >= m.
-__device__ __forceinline__ float rescale_to(float m, float top) { return exp2_approx((m - (top == -INFINITY ? 0.f : top)) * kLog2e); }
 
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -346,7 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        const long long label = live ? __ldg(a.labels + row) - col0 : -1;  // within this slice?
+        long long label = live ? __ldg(a.labels + row) - col0 : -1;  // within this slice?
+        if (label >= width) label = -1;
         // one 32-column piece of the row's logits; columns past the vocabulary become -inf
         auto logits = [&](int c, float (&z)[32]) {
           uint32_t v[32];
@@ -367,31 +350,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               z[j] = c + j < width ? __uint_as_float(v[j]) + (a.bias ? __ldg(a.bias + col0 + c + j) : 0.f) : -INFINITY;
           }
         };
-        auto keep_label = [&](int c, const float (&z)[32]) {
-          if (__any_sync(0xffffffffu, label >= c && label < c + 32)) {
-            float at = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) at = (label == c + j) ? z[j] : at;
-            if (label >= c && label < c + 32 && label < width) a.label_logit[row] = at;
-          }
-        };
         float m = -INFINITY, sum = 0.f;
         if constexpr (MODE == kLoss) {
 #pragma unroll 1
           for (int c = 0; c < kSlice; c += 32) {
             float z[32];
             logits(c, z);
-            float top = z[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
-            top = fmaxf(top, m);
-            keep_label(c, z);
-            exp_from(z, top);
-            float part = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) part += z[j];
-            sum = fmaf(sum, rescale_to(m, top), part);
-            m = top;
+            keep_label(z, label, c, a.label_logit + row);
+            take_into(z, m, sum);
           }
         } else {
 #pragma unroll 1
@@ -400,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             logits(c, z);
 #pragma unroll
             for (int j = 0; j < 32; ++j) m = fmaxf(m, z[j]);
-            keep_label(c, z);
+            keep_label(z, label, c, a.label_logit + row);
           }
           unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
 #pragma unroll 1
@@ -493,7 +459,7 @@ __global__ void __launch_bounds__(1024)
 // vocabulary that is not ignore_index gives NaN (and NaN gradients): loud, and nothing is read out of bounds.
 __global__ void __launch_bounds__(1024)
     xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
-                       const long long* __restrict__ labels, long long ignore_index, long long rows, long long vocab,
+                       const long long* __restrict__ labels, long long label_period, long long ignore_index, long long rows, long long vocab,
                        float2* __restrict__ norm, float* __restrict__ loss) {
   __shared__ float sm[32][33], ss[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -515,7 +481,7 @@ __global__ void __launch_bounds__(1024)
     const float base = m == -INFINITY ? 0.f : m;
     s = 0.f;
     for (int w = 0; w < 32; ++w) s += ss[w][lane] * expf(sm[w][lane] - base);
-    const long long y = labels[row];
+    const long long y = labels[row % label_period];
     const bool ignored = y == ignore_index, outside = !ignored && (y < 0 || y >= vocab);
     if (norm) norm[row] = make_float2(m, outside ? NAN : 1.0f / s);
     loss[row] = ignored ? 0.f : (outside ? NAN : (m - label_logit[row]) + logf(s));
@@ -839,15 +805,6 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
   return launch_product<MODE, false, false, FP16>(map_a, map_b, a, x.stream);
 }
 
-template <bool FP16>
-int finish_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats, float2* norm, float* loss) {
-  const int slices = (int)((x.vocab + kSlice - 1) / kSlice);
-  xent_finish_kernel<<<(unsigned)((n + 31) / 32), 1024, 0, x.stream>>>(b.stats, ld_stats, slices, b.label_logit, x.labels + r0,
-                                                                     x.ignore_index, n, x.vocab, norm, loss + r0);
-  EVOX_LAUNCH_CHECK();
-  return EVOX_OK;
-}
-
 // out (M x N, 16 bits, dense) = scale * A B^T with the reduction divided where that fills the machine better.
 // `sum`: running 32-bit sum over row chunks (null: this product is the whole); `first`, `last`: which chunk.
 template <bool A_MN, bool FP16>
@@ -893,7 +850,8 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     const long long n = x.rows - r0 < chunk ? x.rows - r0 : chunk;
     const bool first = r0 == 0, last = r0 + n == x.rows;
     if (int rc = logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
-    if (int rc = finish_pass<FP16>(x, b, r0, n, chunk, b.norm, b.loss)) return rc;
+    if (int rc = xent_finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, b.loss + r0, x.stream))
+      return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
     const int column_blocks = (int)((x.vocab + 1023) / 1024), row_blocks = (int)((n + 127) / 128);
     xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (dw ? 1 : 0))), 256, 0, x.stream>>>(
@@ -926,6 +884,16 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
 }
 
 }  // namespace
+
+int xent_finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
+                long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, cudaStream_t stream) {
+  const int slices = (int)((vocab + kSlice - 1) / kSlice);
+  xent_finish_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(stats, ld_stats, slices, label_logit, labels, label_period,
+                                                                      ignore_index, rows, vocab, norm, loss);
+  EVOX_LAUNCH_CHECK();
+  return EVOX_OK;
+}
+
 }  // namespace evox
 
 using namespace evox;
@@ -950,7 +918,7 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
   EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
   if (int rc = dtype == EVOX_DTYPE_FP16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
   float* per_row = reduction == EVOX_REDUCE_NONE ? loss : b.loss;
-  if (int rc = finish_pass<false>(x, b, 0, rows, rows, nullptr, per_row)) return rc;
+  if (int rc = xent_finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, per_row, s)) return rc;
   if (reduction != EVOX_REDUCE_NONE) {
     xent_weights_kernel<<<1, 1024, 0, s>>>(x.labels, ignore_index, rows, reduction, nullptr, 1.0f, b.scalars);
     EVOX_LAUNCH_CHECK();

@@ -33,6 +33,7 @@
 #include <math.h>
 
 #include "sm100.cuh"
+#include "xent.cuh"
 
 namespace evox {
 namespace {
@@ -99,6 +100,10 @@ struct GemmArgs {
   // different CTAs; with 2 each adds its sum into the zero-filled out_f32 with an atomic add (two addends:
   // the result does not depend on their order).
   int k_split;
+  // Cross entropy (EPI 3): class labels shared by the population, and what the epilogue leaves of the logits
+  const long long* labels;  // [batch]
+  float2* stats;            // [column slice][M]: (maximum, sum of exponentials)
+  float* label_logit;       // [M]
 };
 
 // kind::f16 instruction descriptor: D = fp32, A = B = bf16, both K-major, N = 256, M = 128
@@ -130,7 +135,9 @@ __device__ __forceinline__ float4 normal4(unsigned long long seed, unsigned long
 // EPI: what the layer epilogue does, known at compile time so that none of it is a condition inside the
 // per-element loops. 0: whatever the arguments say; 1: hidden layer of a virtual-LoRA network (rank-8 correction,
 // ReLU, bf16 output, next layer's projection; no bias, no bias noise); 2: its last layer (rank-8 correction, squared
-// error against the target; no bias, no bias noise, no ReLU). The accumulate variant ignores it.
+// error against the target; no bias, no bias noise, no ReLU); 3: its last layer as a vocabulary head (any number of
+// columns, bias and bias noise as the arguments say): the softmax statistics of each row's 128 columns and the label's
+// logit instead of the logits. The accumulate variant ignores it.
 template <bool PAIR, bool ACCUM, int EPI = 0>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const GemmArgs a) {
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffBars + 8 * (2 * STAGES + 4));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long n_tiles_n = a.N / BN;
+  const long long n_tiles_n = EPI == 3 ? (a.N + BN - 1) / BN : a.N / BN;
   const long long n_tiles = (a.M / TM) * n_tiles_n;
   // a CTA pair walks the tile list together; each CTA owns 128 of the tile's 256 rows
   const uint32_t cta_rank = PAIR ? cluster_rank() : 0u;
@@ -395,12 +402,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const long long p_first = m0 / a.batch;
       // what this epilogue does: compile-time constants for the two fixed shapes, the arguments otherwise
       const bool has_t = EPI != 0 ? true : a.t != nullptr;
-      const bool has_bias = EPI != 0 ? false : a.bias != nullptr;
-      const bool has_noise = EPI != 0 ? false : a.has_bias_noise != 0;
-      const bool do_relu = EPI == 1 ? true : (EPI == 2 ? false : a.relu != 0);
-      const bool to_target = EPI == 2 ? true : (EPI == 1 ? false : a.target != nullptr);
-      const bool to_bf16 = EPI == 1 ? true : (EPI == 2 ? false : a.out_bf16 != nullptr);
-      const bool project = EPI == 1 ? true : (EPI == 2 ? false : a.t_partial != nullptr);
+      const bool has_bias = EPI == 0 || EPI == 3 ? a.bias != nullptr : false;
+      const bool has_noise = EPI == 0 || EPI == 3 ? a.has_bias_noise != 0 : false;
+      const bool do_relu = EPI == 1 ? true : (EPI >= 2 ? false : a.relu != 0);
+      const bool to_target = EPI == 2 ? true : (EPI != 0 ? false : a.target != nullptr);
+      const bool to_bf16 = EPI == 1 ? true : (EPI >= 2 ? false : a.out_bf16 != nullptr);
+      const bool project = EPI == 1 ? true : (EPI >= 2 ? false : a.t_partial != nullptr);
       // all epilogue threads are done with the previous tile's factors
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (has_t) {
@@ -467,6 +474,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int q = 0; q < RANK; ++q) tp[q] = 0.f;
       const float* target_row = to_target ? a.target + (row % a.batch) * a.N + n0 : nullptr;
       float sq_sum = 0.f;
+      float top = -INFINITY, exp_sum = 0.f;  // EPI 3
+      const long long slice0 = n0 + col_half * (BN / 2);
+      const int width = EPI == 3 ? (int)max(0ll, min(a.N - slice0, (long long)(BN / 2))) : BN / 2;  // columns that exist
+      long long label = EPI == 3 ? __ldg(a.labels + row % a.batch) - slice0 : -1;
+      if (label >= width) label = -1;
       for (int c = col_half * (BN / 2); c < (col_half + 1) * (BN / 2); c += 32) {
         uint32_t v[32];
         tmem_ld32(tmem_base + (uint32_t)(buf * BN + c) + ((uint32_t)(quarter * 32) << 16), v);
@@ -475,7 +487,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           float acc = __uint_as_float(v[j]) * a.out_scale;
-          if (has_bias) acc += __ldg(a.bias + n0 + c + j);
+          if constexpr (EPI == 3) {
+            if (has_bias && c - col_half * (BN / 2) + j < width) acc += __ldg(a.bias + n0 + c + j);
+          } else {
+            if (has_bias) acc += __ldg(a.bias + n0 + c + j);
+          }
           if (has_t) {
             const float4 b0 = *reinterpret_cast<const float4*>(bf + (size_t)(c + j) * RANK);
             const float4 b1 = *reinterpret_cast<const float4*>(bf + (size_t)(c + j) * RANK + 4);
@@ -492,7 +508,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           if (has_noise) acc = fmaf(a.sigma, bn[c + j], acc);
           y[j] = do_relu ? fmaxf(acc, 0.f) : acc;
         }
-        if (to_target) {
+        if constexpr (EPI == 3) {
+          const int at = c - col_half * (BN / 2);
+          if (at + 32 > width) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = at + j < width ? y[j] : -INFINITY;
+          }
+          keep_label(y, label, at, a.label_logit + row);
+          take_into(y, top, exp_sum);
+          __syncwarp();
+        } else if (to_target) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 tg = __ldg(reinterpret_cast<const float4*>(target_row + c + j));
@@ -540,6 +565,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
+      if (EPI == 3 && width > 0) a.stats[(slice0 / kSlice) * a.M + row] = make_float2(top, exp_sum);
       if (to_target) a.row_partial[(row * n_tiles_n + n_blk) * 2 + col_half] = sq_sum;
       if (project && to_bf16) {
         float* o = a.t_partial + ((size_t)row * (size_t)(n_tiles_n * 2) + (size_t)(n_blk * 2 + col_half)) * RANK;
@@ -853,7 +879,7 @@ int launch_gemm(const void* a_base, long long a_rows, const void* b_base, long l
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
-  const long long n_tiles = (a.M / (pair ? 2 * BM : BM)) * (a.N / BN);
+  const long long n_tiles = (a.M / (pair ? 2 * BM : BM)) * ((a.N + BN - 1) / BN);
   const long long slots = pair ? sm_count() / 2 : sm_count();
   a.k_split = 1;
   if (accumulate) {
@@ -881,6 +907,8 @@ int launch_gemm(const void* a_base, long long a_rows, const void* b_base, long l
   int rc;
   if (accumulate)
     rc = pair ? launch_variant<true, true>(cfg, map_a, map_b, a) : launch_variant<false, true>(cfg, map_a, map_b, a);
+  else if (a.labels != nullptr)
+    rc = pair ? launch_variant<true, false, 3>(cfg, map_a, map_b, a) : launch_variant<false, false, 3>(cfg, map_a, map_b, a);
   else if (pair && hidden)
     rc = launch_variant<true, false, 1>(cfg, map_a, map_b, a);
   else if (pair && last)
@@ -956,10 +984,58 @@ extern "C" int evox_lora_gemm_bf16(const void* h, const void* w, const float* bi
   a.out_scale_dev = nullptr;
   for (int c = 0; c < 6; ++c) a.combo_scale[c] = 1.0f;
   a.t_partial = t_next_partial;
+  a.labels = nullptr;
   a.next_a_counter = next_a_counter;
   EVOX_REQUIRE(t_next_partial == nullptr || out_bf16 != nullptr, EVOX_ERR_INVALID,
                "lora_gemm_bf16: the fused next-layer projection needs the bf16 output sink");
   return launch_gemm(h, a.M, w, d, k, a, false, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int evox_lora_cross_entropy_supported(int64_t pop, int64_t batch, int64_t k, int64_t vocab, int32_t r) {
+  // the layer's rules with any number of columns; the first projection takes the input in pieces of 128 columns
+  return vocab > 0 && vocab < (1ll << 26) && k % 128 == 0 && evox_lora_gemm_supported(pop, batch, k, BN, r) ? 1 : 0;
+}
+
+extern "C" size_t evox_lora_cross_entropy_workspace_bytes(int64_t pop, int64_t batch, int64_t vocab) {
+  if (pop <= 0 || batch <= 0 || vocab <= 0) return 0;
+  return (size_t)(pop * batch) * (sizeof(float2) * (size_t)((vocab + kSlice - 1) / kSlice) + sizeof(float));
+}
+
+extern "C" int evox_lora_cross_entropy_bf16(const void* h, const void* w, const float* bias, const float* t, const int64_t* seeds,
+                                            uint64_t b_counter, int32_t has_bias_noise, uint64_t noise_counter, float sigma, int64_t pop,
+                                            int64_t batch, int64_t k, int64_t vocab, int32_t r, const int64_t* labels, int64_t ignore_index,
+                                            float* loss, void* workspace, size_t workspace_bytes, int32_t* error_flag, void* stream) {
+  EVOX_REQUIRE(h && w && t && seeds && labels && loss && workspace && error_flag, EVOX_ERR_INVALID, "lora_cross_entropy: NULL pointer");
+  EVOX_REQUIRE(evox_lora_cross_entropy_supported(pop, batch, k, vocab, r), EVOX_ERR_INVALID,
+               "lora_cross_entropy: shape (pop %lld, batch %lld, k %lld, vocab %lld, r %d) is not supported", (long long)pop, (long long)batch,
+               (long long)k, (long long)vocab, r);
+  EVOX_REQUIRE(aligned16(h) && aligned16(w) && aligned16(t), EVOX_ERR_INVALID, "lora_cross_entropy: operands must be 16-byte aligned");
+  EVOX_REQUIRE(((uintptr_t)workspace & 15u) == 0, EVOX_ERR_INVALID, "lora_cross_entropy: workspace must be 16-byte aligned");
+  EVOX_REQUIRE(workspace_bytes >= evox_lora_cross_entropy_workspace_bytes(pop, batch, vocab), EVOX_ERR_WORKSPACE, "lora_cross_entropy: workspace too small");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  GemmArgs a = {};
+  a.M = pop * batch;
+  a.N = vocab;
+  a.K = k;
+  a.batch = batch;
+  a.bias = bias;
+  a.t = t;
+  a.seeds = (const long long*)seeds;
+  a.b_counter = b_counter;
+  a.noise_counter = noise_counter;
+  a.has_bias_noise = has_bias_noise;
+  a.sigma = sigma;
+  a.error_flag = error_flag;
+  a.n_combo = 1;
+  a.out_scale = 1.0f;
+  a.k_split = 1;
+  a.operand_format = kFormatBf16;
+  a.labels = (const long long*)labels;
+  a.stats = reinterpret_cast<float2*>(workspace);
+  a.label_logit = reinterpret_cast<float*>(a.stats + a.M * ((vocab + kSlice - 1) / kSlice));
+  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
+  if (int rc = launch_gemm(h, a.M, w, vocab, k, a, false, s)) return rc;
+  return xent_finish(a.stats, a.M, a.label_logit, a.labels, batch, ignore_index, a.M, vocab, nullptr, loss, s);
 }
 
 extern "C" int evox_neg_mse_from_partials(const float* row_partial, int64_t pop, int64_t batch, int64_t d, float* fitness,
@@ -1062,6 +1138,7 @@ extern "C" int evox_lora_gradient_tc(const float* fitness, const int64_t* seeds,
     a.out_scale_dev = nullptr;
   }
   a.t_partial = nullptr;
+  a.labels = nullptr;
   a.next_a_counter = 0;
   a.out_scale = 1.0f / ((float)pop * sigma);
   a.ld_out = k;

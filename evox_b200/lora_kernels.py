@@ -14,7 +14,7 @@ from . import _cabi
 
 __all__ = [
     "philox_uniform", "philox_normal", "compute_counter_offsets", "generate_lora_factors",
-    "lora_delta_output", "lora_gradient", "lora_gradient_from_seeds", "lora_layer_bf16", "raise_on_kernel_errors",
+    "lora_delta_output", "lora_gradient", "lora_gradient_from_seeds", "lora_layer_bf16", "lora_layer_cross_entropy", "raise_on_kernel_errors",
 ]
 
 _grad_ws: dict[torch.device, torch.Tensor] = {}
@@ -34,6 +34,15 @@ def raise_on_kernel_errors() -> None:
         code = int(flag)
         if code != 0:
             raise _cabi.EvoxKernelError(f"{what}: the tensor-core kernel gave up with status {code} (a bounded wait expired)")
+
+
+def kernel_flag(what: str, dev: torch.device) -> torch.Tensor:
+    """A status word for one tensor-core launch that sets it itself, remembered for `raise_on_kernel_errors`."""
+    err = torch.empty(1, dtype=torch.int32, device=dev)
+    if not torch.cuda.is_current_stream_capturing():  # a captured launch's flag belongs to the graph's replays
+        _pending_flags.append((what, err))
+        del _pending_flags[:-256]
+    return err
 
 
 def _seeds(seeds: torch.Tensor) -> torch.Tensor:
@@ -192,6 +201,52 @@ def lora_layer_bf16(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tensor, count
         _cabi.check(lib.evox_lora_t_from_partials(_cabi.ptr(t_partial), pop * batch, d, _cabi.ptr(t_next), s))
         return out_bf16, t_next
     return out_bf16 if out_bf16 is not None else out_f32
+
+
+def lora_layer_cross_entropy(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tensor, counter: int, sigma: float, labels: torch.Tensor, *,
+                             bias: torch.Tensor | None = None, bias_counter: int | None = None, t: torch.Tensor | None = None,
+                             ignore_index: int = -100) -> torch.Tensor:
+    """Cross entropy of a virtual-LoRA vocabulary head on the tensor cores: the losses (pop, batch), fp32, of
+    `lora_layer_bf16`'s layer (same arguments; w (vocab, k) of any vocab) against class `labels` (batch,) shared by the population.
+    The epilogue reduces the logits to softmax statistics, so (pop, batch, vocab) never exists. A token labelled `ignore_index`
+    has loss 0, another label outside the vocabulary gives NaN."""
+    rank = 8
+    if h.ndim != 3 or w.ndim != 2 or h.shape[2] != w.shape[1]:
+        raise _cabi.EvoxKernelError(f"shape mismatch: h {tuple(h.shape)}, w {tuple(w.shape)}")
+    pop, batch, k = h.shape
+    vocab = w.shape[0]
+    dev = h.device
+    if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise _cabi.EvoxKernelError("lora_layer_cross_entropy needs bf16 activations and weights")
+    seeds = _seeds(seeds)
+    if seeds.shape[0] != pop or labels.dtype != torch.int64 or labels.shape != (batch,):
+        raise _cabi.EvoxKernelError(f"needs {pop} seeds and int64 labels of shape ({batch},), got {seeds.shape[0]} and {labels.dtype} {tuple(labels.shape)}")
+    if bias is not None and bias.shape != (vocab,):
+        raise _cabi.EvoxKernelError(f"bias must have shape ({vocab},), got {tuple(bias.shape)}")
+    if t is not None and (t.shape != (pop, batch, rank) or t.dtype != torch.float32):
+        raise _cabi.EvoxKernelError(f"t must be fp32 of shape ({pop}, {batch}, {rank}), got {t.dtype} {tuple(t.shape)}")
+    if not _cabi.lib.evox_lora_cross_entropy_supported(pop, batch, k, vocab, rank):
+        raise _cabi.EvoxKernelError(f"layer shape (pop {pop}, batch {batch}, k {k}, vocab {vocab}) is not supported by the tensor-core path")
+    h, w, labels = h.contiguous(), w.contiguous(), labels.contiguous()
+    lib, s = _cabi.lib, _cabi.stream_ptr(dev)
+    if t is not None:
+        t = t.contiguous()
+    else:
+        t = torch.empty(pop, batch, rank, dtype=torch.float32, device=dev)
+        _cabi.check(lib.evox_lora_down_bf16(_cabi.ptr(h), _cabi.ptr(seeds), counter, pop, batch, k, rank, _cabi.ptr(t), s))
+    bias_f = None if bias is None else bias.to(device=dev, dtype=torch.float32).contiguous()
+    loss = torch.empty(pop, batch, dtype=torch.float32, device=dev)
+    nbytes = lib.evox_lora_cross_entropy_workspace_bytes(pop, batch, vocab)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    err = kernel_flag("lora_layer_cross_entropy", dev)
+    _cabi.check(
+        lib.evox_lora_cross_entropy_bf16(
+            _cabi.ptr(h), _cabi.ptr(w), _cabi.ptr(bias_f), _cabi.ptr(t), _cabi.ptr(seeds), counter + _ceil4(rank * k),
+            int(bias is not None and bias_counter is not None), bias_counter or 0, float(sigma), pop, batch, k, vocab, rank,
+            _cabi.ptr(labels), ignore_index, _cabi.ptr(loss), _cabi.ptr(ws), nbytes, _cabi.ptr(err), s,
+        )
+    )
+    return loss
 
 
 def lora_gradient_from_seeds(fitness: torch.Tensor, seeds: torch.Tensor, weight_shape: tuple, rank: int, counter: int,

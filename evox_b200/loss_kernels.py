@@ -12,7 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _cabi
-from .lora_kernels import _pending_flags
+from .lora_kernels import kernel_flag
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_grad"]
 
@@ -63,14 +63,6 @@ def _pointer(x: torch.Tensor, name: str) -> int:
     return x.data_ptr()
 
 
-def _flag(what: str, dev: torch.device) -> torch.Tensor:
-    err = torch.empty(1, dtype=torch.int32, device=dev)
-    if not torch.cuda.is_current_stream_capturing():  # a captured launch's flag belongs to the graph's replays
-        _pending_flags.append((what, err))
-        del _pending_flags[:-256]
-    return err
-
-
 def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
     dev = h.device
     rows, hidden = h.shape
@@ -82,7 +74,7 @@ def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
     lib = _cabi.lib
     nbytes = lib.evox_linear_cross_entropy_workspace_bytes(rows, hidden, vocab)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = _flag("linear_cross_entropy", dev)
+    err = kernel_flag("linear_cross_entropy", dev)
     _cabi.check(lib.evox_linear_cross_entropy(
         _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
         ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(loss), _cabi.ptr(ws), nbytes, _cabi.ptr(err),
@@ -106,7 +98,7 @@ def _loss_and_grad(h, weight, labels, bias, ignore_index, reduction, shape, grad
     chunk = lib.evox_linear_cross_entropy_chunk_rows(rows, vocab) if chunk_rows is None else chunk_rows
     nbytes = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, hidden, vocab, chunk, db is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = _flag("linear_cross_entropy_grad", dev)
+    err = kernel_flag("linear_cross_entropy_grad", dev)
     _cabi.check(lib.evox_linear_cross_entropy_grad(
         _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
         ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(grad_loss), chunk, _cabi.ptr(loss), _cabi.ptr(dh),

@@ -13,12 +13,15 @@ from typing import Optional, Sequence
 import torch
 
 from . import _cabi
+from . import grad_kernels as _gk
 from . import lora_kernels as _lk
+from . import loss_kernels as _loss
 from .operators import selection as _sel
 
 __all__ = ["nd_rank", "crowding_distance", "nd_environmental_selection", "ref_vec_guided", "philox_uniform", "philox_normal",
            "lora_delta_output", "lora_gradient", "eval_fitness", "pso_step", "pso_generation", "openes_ask", "openes_gradient",
-           "es_update", "offspring", "lora_layer", "lora_layer_next", "lora_layer_neg_mse", "lora_gradient_seeds"]
+           "es_update", "offspring", "lora_layer", "lora_layer_next", "lora_layer_neg_mse", "lora_gradient_seeds",
+           "linear_cross_entropy", "linear_cross_entropy_grad", "lora_layer_cross_entropy", "grad_norm", "clip_grad_norm_"]
 
 
 @torch.library.custom_op("evox_b200::nd_rank", mutates_args=(), device_types="cuda")
@@ -319,6 +322,71 @@ def lora_gradient_seeds(fitness: torch.Tensor, seeds: torch.Tensor, d: int, k: i
 @lora_gradient_seeds.register_fake
 def _(fitness, seeds, d, k, rank, counter, pop_size, sigma, passes):
     return fitness.new_empty(d, k, dtype=torch.float32)
+
+
+@torch.library.custom_op("evox_b200::linear_cross_entropy", mutates_args=(), device_types="cuda")
+def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: Optional[torch.Tensor], ignore_index: int,
+                         reduction: str) -> torch.Tensor:
+    """Cross entropy of a linear vocabulary head without its logits (evox_linear_cross_entropy)."""
+    return _loss.linear_cross_entropy(h.detach(), weight.detach(), labels, None if bias is None else bias.detach(),
+                                      ignore_index=ignore_index, reduction=reduction)
+
+
+@linear_cross_entropy.register_fake
+def _(h, weight, labels, bias, ignore_index, reduction):
+    return h.new_empty(labels.shape if reduction == "none" else (), dtype=torch.float32)
+
+
+@torch.library.custom_op("evox_b200::linear_cross_entropy_grad", mutates_args=(), device_types="cuda")
+def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: Optional[torch.Tensor],
+                              grad_loss: Optional[torch.Tensor], ignore_index: int,
+                              reduction: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Loss, dh, dweight and dbias (empty without a bias) in one call (evox_linear_cross_entropy_grad)."""
+    loss, dh, dw, db = _loss.linear_cross_entropy_grad(h, weight, labels, bias, ignore_index=ignore_index, reduction=reduction,
+                                                       grad_loss=grad_loss)
+    return loss, dh, dw, h.new_empty(0) if db is None else db
+
+
+@linear_cross_entropy_grad.register_fake
+def _(h, weight, labels, bias, grad_loss, ignore_index, reduction):
+    return (h.new_empty(labels.shape if reduction == "none" else (), dtype=torch.float32), h.new_empty(h.shape),
+            weight.new_empty(weight.shape), h.new_empty(0) if bias is None else bias.new_empty(bias.shape))
+
+
+@torch.library.custom_op("evox_b200::lora_layer_cross_entropy", mutates_args=(), device_types="cuda")
+def lora_layer_cross_entropy(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tensor, counter: int, sigma: float, labels: torch.Tensor,
+                             bias: Optional[torch.Tensor], bias_counter: Optional[int], t: Optional[torch.Tensor],
+                             ignore_index: int) -> torch.Tensor:
+    """Vocabulary head of a virtual-LoRA population fused with the loss: (pop, batch) cross entropies, logits never written."""
+    return _lk.lora_layer_cross_entropy(h, w, seeds, counter, sigma, labels, bias=bias, bias_counter=bias_counter, t=t,
+                                        ignore_index=ignore_index)
+
+
+@lora_layer_cross_entropy.register_fake
+def _(h, w, seeds, counter, sigma, labels, bias, bias_counter, t, ignore_index):
+    return h.new_empty(h.shape[0], h.shape[1], dtype=torch.float32)
+
+
+@torch.library.custom_op("evox_b200::grad_norm", mutates_args=(), device_types="cuda")
+def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
+    """2-norm over all elements of a list of gradients (evox_clip_grad_norm without the scaling)."""
+    return _gk.grad_norm(tensors)
+
+
+@grad_norm.register_fake
+def _(tensors):
+    return tensors[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.custom_op("evox_b200::clip_grad_norm_", mutates_args=("tensors",), device_types="cuda")
+def clip_grad_norm_(tensors: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """Gradients scaled in place to at most `max_norm`; returns the norm they had (evox_clip_grad_norm)."""
+    return _gk.clip_grad_norm_(tensors, max_norm)
+
+
+@clip_grad_norm_.register_fake
+def _(tensors, max_norm):
+    return tensors[0].new_empty((), dtype=torch.float32)
 
 
 # ---------------------------------------------------------------------------------------------

@@ -17,7 +17,9 @@ from torch import nn
 
 from .. import _cabi
 from ..core import Problem
-from ..lora_kernels import compute_counter_offsets, generate_lora_factors, lora_layer_bf16, raise_on_kernel_errors
+from ..lora_kernels import (
+    compute_counter_offsets, generate_lora_factors, lora_layer_bf16, lora_layer_cross_entropy, raise_on_kernel_errors,
+)
 from ..sharding import group_info, shard_bounds
 
 __all__ = ["VirtualLoRAProblem"]
@@ -31,7 +33,10 @@ class VirtualLoRAProblem(Problem):
                  shard: bool = False, group=None):
         """`compute_dtype=torch.bfloat16` runs every Linear layer whose shape the tensor-core kernel
         supports (rank 8, batch 64 or 128 per individual, feature sizes multiples of 256) with bf16
-        operands and fp32 accumulation; other layers and the default use the fp32 kernels."""
+        operands and fp32 accumulation; other layers and the default use the fp32 kernels. A last Linear layer on
+        that path ends in the loss itself, without storing its outputs, for `nn.MSELoss(reduction="none")` and, as
+        a vocabulary head of any number of classes, for `nn.CrossEntropyLoss(reduction="none")` without class
+        weights or label smoothing."""
         super().__init__()
         self.compute_dtype = compute_dtype
         # shard=True: this rank evaluates only its tensor_split share of the individuals and the
@@ -71,10 +76,11 @@ class VirtualLoRAProblem(Problem):
         return center[self._starts[i] : self._starts[i] + n].view(self.param_shapes[i]), i
 
     def _virtual_forward(self, inputs: torch.Tensor, center: torch.Tensor, seeds: torch.Tensor, sigma: float, pop_size: int,
-                         mse_target: torch.Tensor | None = None):
+                         mse_target: torch.Tensor | None = None, class_labels: torch.Tensor | None = None, ignore_index: int = -100):
         """Activations of the last layer, (pop, batch, out) fp32. With `mse_target` (batch, out) and a
         last Linear layer on the tensor-core path, the squared error is reduced inside that layer's
-        epilogue and a `("mse", per-individual mean squared error)` tuple is returned instead."""
+        epilogue and a `("mse", per-individual mean squared error)` tuple is returned instead; with
+        `class_labels` (batch,), such a last layer ends in the cross entropy: `("cross_entropy", losses (pop, batch))`."""
         dev = center.device
         shared = inputs.ndim == 2
         h = inputs.to(device=dev).contiguous()
@@ -93,6 +99,15 @@ class VirtualLoRAProblem(Problem):
                 weight, wi = self._param(center, f"{name}.weight")
                 d, k = weight.shape
                 relu = pos + 1 < len(children) and isinstance(children[pos + 1][1], nn.ReLU)
+                if (class_labels is not None and pos + 1 == len(children) and self.compute_dtype == torch.bfloat16 and not shared
+                        and lib.evox_lora_cross_entropy_supported(pop_size, batch, k, d, self.lora_rank)):
+                    bias = bias_counter = None
+                    if module.bias is not None:
+                        bias, bi = self._param(center, f"{name}.bias")
+                        bias_counter = self.counter_offsets[bi]
+                    return "cross_entropy", lora_layer_cross_entropy(
+                        h.to(torch.bfloat16), weight.to(torch.bfloat16), seeds, self.counter_offsets[wi], sigma, class_labels, bias=bias,
+                        bias_counter=bias_counter, t=pending_t, ignore_index=ignore_index)
                 if (self.compute_dtype == torch.bfloat16 and not shared
                         and lib.evox_lora_gemm_supported(pop_size, batch, k, d, self.lora_rank)):
                     bias = bias_counter = None
@@ -110,7 +125,9 @@ class VirtualLoRAProblem(Problem):
                     next_counter = None
                     if not last and isinstance(children[nxt][1], nn.Linear):
                         nd, nk = children[nxt][1].weight.shape
-                        if nk == d and lib.evox_lora_gemm_supported(pop_size, batch, nk, nd, self.lora_rank):
+                        head = class_labels is not None and nxt + 1 == len(children)
+                        if nk == d and (lib.evox_lora_gemm_supported(pop_size, batch, nk, nd, self.lora_rank)
+                                        or (head and lib.evox_lora_cross_entropy_supported(pop_size, batch, nk, nd, self.lora_rank))):
                             next_counter = self.counter_offsets[self.param_names.index(f"{children[nxt][0]}.weight")]
                     res = lora_layer_bf16(
                         h.to(torch.bfloat16), weight.to(torch.bfloat16), seeds, self.counter_offsets[wi], sigma, bias=bias,
@@ -191,7 +208,14 @@ class VirtualLoRAProblem(Problem):
                 inputs = inputs[span[0] : span[1]]
             fuse = (isinstance(self.criterion, nn.MSELoss) and self.criterion.reduction == "none" and labels.ndim == 2
                     and self.reduction == "mean")
-            logits = self._virtual_forward(inputs, center, seeds, sigma, pop_size, mse_target=labels if fuse else None)
+            cross = (type(self.criterion) is nn.CrossEntropyLoss and self.criterion.reduction == "none" and self.criterion.weight is None
+                     and self.criterion.label_smoothing == 0.0 and labels.ndim == 1 and labels.dtype == torch.int64)
+            logits = self._virtual_forward(inputs, center, seeds, sigma, pop_size, mse_target=labels if fuse else None,
+                                           class_labels=labels if cross else None,
+                                           ignore_index=self.criterion.ignore_index if cross else -100)
+            if isinstance(logits, tuple) and logits[0] == "cross_entropy":  # one loss per individual and sample
+                per_individual.append(logits[1].mean(dim=1) if self.reduction == "mean" else logits[1].sum(dim=1))
+                continue
             if isinstance(logits, tuple):  # the last layer already reduced (y - target)^2 per individual
                 per_individual.append(logits[1])
                 continue

@@ -604,6 +604,19 @@ int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, i
                                    float* loss, void* dh, void* dw, float* dbias, void* workspace,
                                    size_t workspace_bytes, int32_t* error_flag, void* stream);
 
+/* The loss of a virtual-LoRA population's vocabulary head, z = h W^T + bias + sigma t B_p^T +
+ * sigma * bias_noise_p as in evox_lora_gemm_bf16 (same operands, counters and t = h A_p^T; W is
+ * vocab x k), any vocab: loss (pop x batch) against labels (batch) shared by the population,
+ * conventions of evox_linear_cross_entropy. k must be a multiple of 128. */
+int evox_lora_cross_entropy_supported(int64_t pop, int64_t batch, int64_t k, int64_t vocab, int32_t r);
+size_t evox_lora_cross_entropy_workspace_bytes(int64_t pop, int64_t batch, int64_t vocab);
+int evox_lora_cross_entropy_bf16(const void* h, const void* w, const float* bias, const float* t,
+                                 const int64_t* seeds, uint64_t b_counter, int32_t has_bias_noise,
+                                 uint64_t noise_counter, float sigma, int64_t pop, int64_t batch,
+                                 int64_t k, int64_t vocab, int32_t r, const int64_t* labels,
+                                 int64_t ignore_index, float* loss, void* workspace,
+                                 size_t workspace_bytes, int32_t* error_flag, void* stream);
+
 /* norm (one fp32) = 2-norm over all elements of n_tensors dense tensors; with clip != 0 every element is
  * then multiplied by min(1, max_norm / (norm + 1e-6)) in place (nothing is written when that is 1).
  * address, numel, dtype (EVOX_DTYPE_*): HOST arrays, read before the call returns; address holds device
