@@ -34,17 +34,21 @@ namespace {
 
 constexpr int TM = 256, TN = 256, BK = 64, STAGES = 6;  // one tile of a CTA pair; each CTA holds half of both operands
 constexpr int kThreads = 64 + 256;
+constexpr int kChunkBlocks = 16;  // blocks of the reduction per accumulator of a logit
 constexpr uint32_t kOperandBytes = 128 * BK * 2;
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kOffBars = STAGES * kStageBytes;
-constexpr uint32_t kSmemBytes = kOffBars + 256;
+constexpr uint32_t kOffStage = kOffBars + 256;  // a warp's 32 x 32 values on their way to rows that start anywhere
+constexpr int kStagePitch = 34;
+constexpr uint32_t kSmemBytes = kOffStage + 8 * 32 * kStagePitch * 2;
 
 enum { kLoss = 0, kProb = 1, kOut = 2 };
 
 struct ProductArgs {
   long long M, N;
   int k_blocks;            // of BK
-  int splits;              // the reduction is divided among this many work items per tile
+  int splits;              // the reduction is divided among this many work items per tile (kOut)
+  int chunks;              // accumulators that a tile's reduction is divided among (kLoss, kProb)
   int tiles_m, tiles_n;
   int m_fast, group;       // tiles run through `group` of the one direction, then all of the other
   uint32_t idesc;
@@ -56,12 +60,13 @@ struct ProductArgs {
   long long ld_stats;
   float* label_logit;      // [M]
   void* e;                 // [M][ld_e], kProb
+  void* e_low;             // what the rounding of e left, or null
   long long ld_e;
   // kOut
   void* out16;             // [M][ld_out] (final), or null
   float* out32;            // [splits][M][ld32] partial sums, or the running sum over row chunks, or null
   long long ld_out, ld32;
-  int vec16;               // rows of out16 start on 16-byte boundaries
+  int vec16;               // rows of out16 start on 32-byte boundaries
   int add32;               // add what out32 holds before storing (or to out16)
   const float* scale;      // device scalar
 };
@@ -85,6 +90,21 @@ template <bool FP16>
 __device__ __forceinline__ float2 unpack2(uint32_t p) {
   if constexpr (FP16) return __half22float2(*reinterpret_cast<const __half2*>(&p));
   else return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+// Sixteen of a thread's values, from z[j] on, as 16 bits to a 32-byte aligned place.
+template <bool FP16>
+__device__ __forceinline__ void store_packed16(unsigned short* to, const float (&z)[32], int j, float scale) {
+  uint32_t p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = pack2<FP16>(z[j + 2 * i] * scale, z[j + 2 * i + 1] * scale);
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
+               "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
+               : "memory");
+}
+template <bool FP16>
+__device__ __forceinline__ void store_packed(unsigned short* to, const float (&z)[32], float scale) {
+  store_packed16<FP16>(to, z, 0, scale);
+  store_packed16<FP16>(to + 16, z, 16, scale);
 }
 template <bool FP16>
 constexpr float kProbScale = FP16 ? 32768.0f : 1.0f;
@@ -134,9 +154,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t cta_rank = cluster_rank();
   const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
   const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
-  auto kb_range = [&](int split, int& kb0, int& kb1) {
-    kb0 = (int)((long long)split * a.k_blocks / a.splits);
-    kb1 = (int)((long long)(split + 1) * a.k_blocks / a.splits);
+  // a tile's reduction goes to `splits` work items, or through `chunks` accumulators one after the other
+  const int chunks = MODE == kOut ? 1 : a.chunks;
+  auto kb_range = [&](int split, int chunk, int& kb0, int& kb1) {
+    const long long part = MODE == kOut ? split : chunk, parts = MODE == kOut ? a.splits : a.chunks;
+    kb0 = (int)(part * a.k_blocks / parts);
+    kb1 = (int)((part + 1) * a.k_blocks / parts);
   };
 
   if (threadIdx.x == 0) {
@@ -146,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 2 * 256);  // the leader's collects both epilogues
+      mbar_init(tempty_bar(b), 2 * 8);  // the leader's collects both epilogues, an arrival per warp
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -170,8 +193,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (long long work = first; work < n_work && ok; work += step) {
         const Tile t = tile_of(a, work);
         const int m0 = t.m * TM + (int)cta_rank * 128, n0 = t.n * TN + (int)cta_rank * 128;
-        int kb0, kb1;
-        kb_range(t.split, kb0, kb1);
+        const int kb0 = MODE == kOut ? (int)((long long)t.split * a.k_blocks / a.splits) : 0;
+        const int kb1 = MODE == kOut ? (int)((long long)(t.split + 1) * a.k_blocks / a.splits) : a.k_blocks;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) {
             ok = false;
@@ -232,35 +255,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0;
       long long it = 0;
       bool ok = true;
-      for (long long work = first; work < n_work && ok; work += step, ++it) {
+      for (long long work = first; work < n_work && ok; work += step) {
         const Tile t = tile_of(a, work);
-        int kb0, kb1;
-        kb_range(t.split, kb0, kb1);
-        const int buf = (int)(it & 1);
-        if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) break;
-        fence_after_sync();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(buf * TN);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
+        for (int chunk = 0; chunk < chunks && ok; ++chunk, ++it) {
+          int kb0, kb1;
+          kb_range(t.split, chunk, kb0, kb1);
+          const int buf = (int)(it & 1);
+          if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) {
             ok = false;
             break;
           }
           fence_after_sync();
-          const uint32_t sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
+          const uint32_t d_tmem = tmem_base + (uint32_t)(buf * TN);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
+              ok = false;
+              break;
+            }
+            fence_after_sync();
+            const uint32_t sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            // 16 reduction indices further: 32 bytes along a K-major line, 16 lines of an MN-major tile
-            const unsigned long long da = A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32);
-            const unsigned long long db = B_MN ? umma_desc_mn(sb + k * 2048) : umma_desc(sb + k * 32);
-            umma_f16_pair(d_tmem, da, db, a.idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              // 16 reduction indices further: 32 bytes along a K-major line, 16 lines of an MN-major tile
+              const unsigned long long da = A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32);
+              const unsigned long long db = B_MN ? umma_desc_mn(sb + k * 2048) : umma_desc(sb + k * 32);
+              umma_f16_pair(d_tmem, da, db, a.idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+            }
+            umma_commit_pair(empty_bar(s));  // stage reusable in both CTAs once these products have read it
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
-          umma_commit_pair(empty_bar(s));  // stage reusable in both CTAs once these products have read it
-          if (++s == STAGES) {
-            s = 0;
-            ph ^= 1u;
-          }
+          if (ok) umma_commit_pair(tfull_bar(buf));  // accumulator complete
         }
-        if (ok) umma_commit_pair(tfull_bar(buf));  // accumulator complete
       }
     }
   } else {
@@ -269,133 +297,163 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half = (warp - 2) >> 2;      // which 128 of the tile's 256 columns this warp handles
     const uint32_t leader_tempty0 = map_to_cta(tempty_bar(0), 0u);
     long long it = 0;
-    for (long long work = first; work < n_work; work += step, ++it) {
+    for (long long work = first; work < n_work; work += step) {
       const Tile t = tile_of(a, work);
-      const int buf = (int)(it & 1);
       const long long row = (long long)t.m * TM + cta_rank * 128 + quarter * 32 + lane;
       const long long col0 = (long long)t.n * TN + half * kSlice;
       const bool live = row < a.M;
       const int width = (int)max(0ll, min((long long)kSlice, a.N - col0));  // columns of this slice that exist
-      const bool ready = mbar_wait(tfull_bar(buf), (uint32_t)((it >> 1) & 1), a.error_flag, 4);
-      if (!__all_sync(0xffffffffu, ready)) break;
-      fence_after_sync();
-      const uint32_t taddr = tmem_base + (uint32_t)(buf * TN + half * kSlice) + ((uint32_t)(quarter * 32) << 16);
+      long long label = -1;  // column of the slice, if it is there
+      if constexpr (MODE != kOut) {
+        if (live) label = __ldg(a.labels + row) - col0;  // on its way while the accumulator fills
+        if (label >= width) label = -1;
+      }
+      float z[4][32];  // this thread's row of the slice
+      bool ready = true;
+      for (int chunk = 0; chunk < chunks; ++chunk, ++it) {
+        const int buf = (int)(it & 1);
+        ready = mbar_wait(tfull_bar(buf), (uint32_t)((it >> 1) & 1), a.error_flag, 4);
+        ready = __all_sync(0xffffffffu, ready);
+        if (!ready) break;
+        fence_after_sync();
+        const uint32_t taddr = tmem_base + (uint32_t)(buf * TN + half * kSlice) + ((uint32_t)(quarter * 32) << 16);
+        if (chunk == 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(taddr + c * 32, reinterpret_cast<uint32_t(&)[32]>(z[c]));
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(taddr + c * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[c][j] += __uint_as_float(v[j]);
+          }
+        }
+        // the accumulator is in registers: one arrival per warp hands it back. Relaxed: what goes back is tensor memory whose
+        // loads are complete, and a release would make the warp wait for its stores of the previous tile
+        // (ncu, 1,003 x 1,000 x 50,021: a fifth of the epilogue's stalls)
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8u * buf);
+      }
+      if (!ready) break;
       if constexpr (MODE == kOut) {
         const float scale = a.scale ? __ldg(a.scale) : 1.0f;
         float* o32 = a.out32 ? a.out32 + ((long long)t.split * a.M + row) * a.ld32 + col0 : nullptr;
         unsigned short* o16 = a.out16 ? reinterpret_cast<unsigned short*>(a.out16) + row * a.ld_out + col0 : nullptr;
+        if (o32 && live) {  // rows of out32 hold a multiple of four columns
 #pragma unroll
-        for (int c = 0; c < kSlice; c += 32) {
-          uint32_t v[32];
-          __syncwarp();
-          tmem_ld32(taddr + c, v);
-          tmem_ld_wait();
-          if (live && o32) {  // rows of out32 hold a multiple of four columns
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
-              if (c + j < width) {
-                float4 r = make_float4(__uint_as_float(v[j]) * scale, __uint_as_float(v[j + 1]) * scale,
-                                       __uint_as_float(v[j + 2]) * scale, __uint_as_float(v[j + 3]) * scale);
+              if (c * 32 + j < width) {
+                float4 r = make_float4(z[c][j] * scale, z[c][j + 1] * scale, z[c][j + 2] * scale, z[c][j + 3] * scale);
                 if (a.add32) {
-                  const float4 b = *reinterpret_cast<const float4*>(o32 + c + j);
+                  const float4 b = *reinterpret_cast<const float4*>(o32 + c * 32 + j);
                   r.x += b.x; r.y += b.y; r.z += b.z; r.w += b.w;
                 }
-                if (!o16) *reinterpret_cast<float4*>(o32 + c + j) = r;
-                v[j] = __float_as_uint(r.x);
-                v[j + 1] = __float_as_uint(r.y);
-                v[j + 2] = __float_as_uint(r.z);
-                v[j + 3] = __float_as_uint(r.w);
+                if (!o16) *reinterpret_cast<float4*>(o32 + c * 32 + j) = r;
+                z[c][j] = r.x; z[c][j + 1] = r.y; z[c][j + 2] = r.z; z[c][j + 3] = r.w;
+              }
+            }
+        }
+        if (o16 && live) {
+          const float s16 = o32 ? 1.0f : scale;
+          if (a.vec16) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (c * 32 + 32 <= width) {
+                store_packed<FP16>(o16 + c * 32, z[c], s16);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; j += 16)  // rows hold a multiple of 16 columns
+                  if (c * 32 + j < width) store_packed16<FP16>(o16 + c * 32 + j, z[c], j, s16);
               }
             }
           }
-          if (live && o16) {
-            const float s16 = o32 ? 1.0f : scale;
+        }
+        if (o16 && !a.vec16) {
+          // rows that start anywhere: 32 x 32 values pass through shared memory and leave row by row, lanes along it
+          const float s16 = o32 ? 1.0f : scale;
+          unsigned short* stage = reinterpret_cast<unsigned short*>(smem_raw + kOffStage) + (warp - 2) * (32 * kStagePitch);
+          unsigned short* tile16 = reinterpret_cast<unsigned short*>(a.out16) + (row - lane) * a.ld_out + col0;
+          const int rows_here = (int)max(0ll, min(32ll, a.M - (row - lane)));
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (a.vec16 && c + j + 8 <= width) {
-                uint4 p;
-                p.x = pack2<FP16>(__uint_as_float(v[j]) * s16, __uint_as_float(v[j + 1]) * s16);
-                p.y = pack2<FP16>(__uint_as_float(v[j + 2]) * s16, __uint_as_float(v[j + 3]) * s16);
-                p.z = pack2<FP16>(__uint_as_float(v[j + 4]) * s16, __uint_as_float(v[j + 5]) * s16);
-                p.w = pack2<FP16>(__uint_as_float(v[j + 6]) * s16, __uint_as_float(v[j + 7]) * s16);
-                *reinterpret_cast<uint4*>(o16 + c + j) = p;
-              } else {
+          for (int c = 0; c < 4; ++c) {
+            __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (c + j + i < width) o16[c + j + i] = pack1<FP16>(__uint_as_float(v[j + i]) * s16);
-              }
-            }
+            for (int j = 0; j < 32; j += 2)
+              *reinterpret_cast<uint32_t*>(stage + lane * kStagePitch + j) = pack2<FP16>(z[c][j] * s16, z[c][j + 1] * s16);
+            __syncwarp();
+            if (c * 32 + lane < width)
+              for (int i = 0; i < rows_here; ++i) tile16[i * a.ld_out + c * 32 + lane] = stage[i * kStagePitch + lane];
           }
         }
       } else {
-        long long label = live ? __ldg(a.labels + row) - col0 : -1;  // within this slice?
-        if (label >= width) label = -1;
-        // one 32-column piece of the row's logits; columns past the vocabulary become -inf
-        auto logits = [&](int c, float (&z)[32]) {
-          uint32_t v[32];
-          __syncwarp();
-          tmem_ld32(taddr + c, v);
-          tmem_ld_wait();
-          if (c + 32 <= width) {
-            if (a.bias) {
+        if (a.bias) {
+          if (width == kSlice && (reinterpret_cast<uintptr_t>(a.bias) & 15u) == 0) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]) + __ldg(a.bias + col0 + c + j);
-            } else {
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
-            }
+              for (int j = 0; j < 32; j += 4) {
+                const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + col0 + c * 32 + j));
+                z[c][j] += b.x; z[c][j + 1] += b.y; z[c][j + 2] += b.z; z[c][j + 3] += b.w;
+              }
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              z[j] = c + j < width ? __uint_as_float(v[j]) + (a.bias ? __ldg(a.bias + col0 + c + j) : 0.f) : -INFINITY;
-          }
-        };
-        float m = -INFINITY, sum = 0.f;
-        if constexpr (MODE == kLoss) {
-#pragma unroll 1
-          for (int c = 0; c < kSlice; c += 32) {
-            float z[32];
-            logits(c, z);
-            keep_label(z, label, c, a.label_logit + row);
-            take_into(z, m, sum);
-          }
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < kSlice; c += 32) {
-            float z[32];
-            logits(c, z);
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) m = fmaxf(m, z[j]);
-            keep_label(z, label, c, a.label_logit + row);
-          }
-          unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
-#pragma unroll 1
-          for (int c = 0; c < kSlice; c += 32) {
-            float z[32];
-            logits(c, z);
-            exp_from(z, m);
-            float part = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) part += z[j];
-            sum += part;
-            if (live && col0 + c < a.ld_e) {  // rows of e hold a multiple of 64 columns
-              constexpr float s = kProbScale<FP16>;
-#pragma unroll
-              for (int j = 0; j < 32; j += 8) {
-                uint4 p;
-                p.x = pack2<FP16>(z[j] * s, z[j + 1] * s);
-                p.y = pack2<FP16>(z[j + 2] * s, z[j + 3] * s);
-                p.z = pack2<FP16>(z[j + 4] * s, z[j + 5] * s);
-                p.w = pack2<FP16>(z[j + 6] * s, z[j + 7] * s);
-                *reinterpret_cast<uint4*>(e + c + j) = p;
-              }
-            }
+              for (int j = 0; j < 32; ++j)
+                if (c * 32 + j < width) z[c][j] += __ldg(a.bias + col0 + c * 32 + j);
           }
         }
-        if (live && width > 0) a.stats[(long long)(t.n * 2 + half) * a.ld_stats + row] = make_float2(m, sum);
+        if (width < kSlice) {  // columns past the vocabulary
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c * 32 + j >= width) z[c][j] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) keep_label(z[c], label, c * 32, a.label_logit + row);
+        float top[4], part[4];  // four chains at once
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = z[c][0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top[c] = fmaxf(top[c], z[c][j]);
+        }
+        const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), -INFINITY);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) exp_from(z[c], m);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          part[c] = z[c][0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) part[c] += z[c][j];
+        }
+        if (live && width > 0)
+          a.stats[(long long)(t.n * 2 + half) * a.ld_stats + row] = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
+        if constexpr (MODE == kProb) {
+          unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (live && col0 + c * 32 < a.ld_e) {  // rows of e hold a multiple of 64 columns
+              store_packed<FP16>(e + c * 32, z[c], kProbScale<FP16>);
+              if (a.e_low) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                  const float2 kept = unpack2<FP16>(pack2<FP16>(z[c][j] * kProbScale<FP16>, z[c][j + 1] * kProbScale<FP16>));
+                  z[c][j] = fmaf(z[c][j], kProbScale<FP16>, -kept.x);
+                  z[c][j + 1] = fmaf(z[c][j + 1], kProbScale<FP16>, -kept.y);
+                }
+                store_packed<FP16>(reinterpret_cast<unsigned short*>(a.e_low) + row * a.ld_e + col0 + c * 32, z[c], 1.0f);
+              }
+            }
+        }
       }
-      fence_before_sync();
-      mbar_arrive_cluster(leader_tempty0 + 8u * buf);  // this thread no longer reads the accumulator
     }
   }
   fence_before_sync();
@@ -488,93 +546,107 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// e -> g in place (see the head of the file), 128 rows x 1,024 columns per block, eight columns per thread; column sums
-// of the block's rows for the bias gradient. The blocks of the last grid row copy the hidden states for the weight
-// gradient, with zeros where the label is ignored: 0 x inf in a padded row must not reach dw.
+// e -> g in place (see the head of the file), `block_rows` (at most 32) rows x 1,024 columns per block, eight columns per
+// thread; column sums of the block's rows for the bias gradient, which is a 32-bit result: they take e with what its
+// rounding left. The blocks of the last grid row copy the hidden states for the weight gradient, with zeros where the
+// label is ignored: 0 x inf in a padded row must not reach dw.
 template <bool FP16>
 __global__ void __launch_bounds__(256)
-    xent_rescale_kernel(unsigned short* __restrict__ e, long long ld_e, const float2* __restrict__ stats, long long ld_stats, int slices,
-                        const float2* __restrict__ norm, const long long* __restrict__ labels, long long ignore_index,
-                        const float* __restrict__ grad_loss, int per_row, const float* __restrict__ scalars, long long rows,
-                        long long vocab, float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h,
-                        long long hidden, unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks) {
-  const long long row0 = (long long)blockIdx.x * 128;
-  const int n_rows = (int)min(128ll, rows - row0);
+    xent_rescale_kernel(unsigned short* __restrict__ e, const unsigned short* __restrict__ e_low, long long ld_e,
+                        const float2* __restrict__ stats, long long ld_stats, int slices, const float2* __restrict__ norm,
+                        const long long* __restrict__ labels, long long ignore_index, const float* __restrict__ grad_loss, int per_row,
+                        const float* __restrict__ scalars, long long rows, int block_rows, long long vocab,
+                        float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h, long long hidden,
+                        unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks) {
+  const long long row0 = (long long)blockIdx.x * block_rows;
+  const int n_rows = (int)min((long long)block_rows, rows - row0);
+  const int tid = threadIdx.x;
   if ((int)blockIdx.y >= column_blocks) {
-    for (long long i = threadIdx.x; i < n_rows * (ld_h_out / 8); i += 256) {
-      const long long r = i / (ld_h_out / 8), c = (i - r * (ld_h_out / 8)) * 8;
-      uint4 p = make_uint4(0u, 0u, 0u, 0u);
-      if (labels[row0 + r] != ignore_index) {
-        const unsigned short* src = h + (row0 + r) * ld_h + c;
-        if (c + 8 <= hidden) {
-          p = *reinterpret_cast<const uint4*>(src);
-        } else {  // the row may end here
+    const int pieces = (int)(ld_h_out / 8);
+    for (int r = 0; r < n_rows; ++r) {
+      const bool keep = labels[row0 + r] != ignore_index;
+      const unsigned short* from = h + (row0 + r) * ld_h;
+      unsigned short* to = h_out + (row0 + r) * ld_h_out;
+      for (int i = tid; i < pieces; i += 256) {
+        const int c = i * 8;
+        uint4 p = make_uint4(0u, 0u, 0u, 0u);
+        if (keep && c + 8 <= hidden) {
+          p = __ldg(reinterpret_cast<const uint4*>(from + c));
+        } else if (keep) {  // the row may end here
           unsigned short* q = reinterpret_cast<unsigned short*>(&p);
           for (int j = 0; j < 8; ++j)
-            if (c + j < hidden) q[j] = src[j];
+            if (c + j < hidden) q[j] = from[c + j];
         }
+        *reinterpret_cast<uint4*>(to + c) = p;
       }
-      *reinterpret_cast<uint4*>(h_out + (row0 + r) * ld_h_out + c) = p;
     }
     return;
   }
-  __shared__ float factor[128][8];
-  __shared__ float weight[128];
-  __shared__ int target[128];
+  __shared__ float factor[32][8];
+  __shared__ float weight[32];
+  __shared__ int target[32];
   __shared__ float sums[128][8];
-  const int tid = threadIdx.x;
   const long long col_base = (long long)blockIdx.y * 1024;
-  const float inverse = scalars[1];
-  if (tid < n_rows) {
-    const long long y = labels[row0 + tid];
-    const bool valid = y != ignore_index;
-    weight[tid] = valid ? (per_row && grad_loss ? grad_loss[row0 + tid] * inverse : 1.0f) : 0.f;
-    const long long d = y - col_base;
-    target[tid] = valid && d >= 0 && d < 1024 ? (int)d : -1;
-  }
-  __syncthreads();
-  for (int i = tid; i < 8 * 128; i += 256) {
-    const int s = i >> 7, r = i & 127;
+  {  // one (row, slice) per thread
+    const int r = tid & 31, s = tid >> 5;
     const long long slice = col_base / kSlice + s;
-    float f = 0.f;
-    if (r < n_rows && slice < slices) {
-      const float m = stats[slice * ld_stats + row0 + r].x;
+    float f = 0.f, w = 0.f;
+    int at = -1;
+    if (r < n_rows) {
+      const long long y = labels[row0 + r], d = y - col_base;
+      if (y != ignore_index) {
+        w = per_row && grad_loss ? grad_loss[row0 + r] * scalars[1] : 1.0f;
+        if (d >= 0 && d < 1024) at = (int)d;
+      }
       // w = 0 (an ignored row) stays 0 whatever the row holds: 0 x NaN is not formed
-      const float2 q = norm[row0 + r];
-      f = weight[r] == 0.f ? 0.f : rescale_to(m, q.x) * q.y * weight[r];
+      if (w != 0.f && slice < slices) {
+        const float2 q = norm[row0 + r];
+        f = rescale_to(stats[slice * ld_stats + row0 + r].x, q.x) * q.y * w;
+      }
     }
     factor[r][s] = f;
+    if (s == 0) {
+      weight[r] = w;
+      target[r] = at;
+    }
   }
   __syncthreads();
-  const int group = tid & 127, part = tid >> 7;  // eight columns; which half of the rows
+  const int group = tid & 127, part = tid >> 7;  // eight columns; even or odd rows
   const long long col = col_base + group * 8;
   float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
   if (col < ld_e) {
-#pragma unroll 4
-    for (int r = part; r < n_rows; r += 2) {
-      uint4* at = reinterpret_cast<uint4*>(e + (row0 + r) * ld_e + col);
-      const float f = factor[r][group >> 4];
-      uint4 p = make_uint4(0u, 0u, 0u, 0u);
-      if (weight[r] != 0.f) {
-        p = *at;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&p);
-        const int t = target[r] - group * 8;
+    unsigned short* column = e + row0 * ld_e + col;
+    auto one = [&](int r, uint4 p) {
+      const float f = factor[r][group >> 4], w = weight[r];
+      uint32_t* word = reinterpret_cast<uint32_t*>(&p);
+      uint4 low = make_uint4(0u, 0u, 0u, 0u);
+      if (bias_partial && w != 0.f) low = __ldcs(reinterpret_cast<const uint4*>(e_low + (row0 + r) * ld_e + col));
+      const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
+      const int t = target[r] - group * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 x = unpack2<FP16>(w[j]);
-          x.x *= f;
-          x.y *= f;
-          if (t == 2 * j) x.x = fmaf(-kProbScale<FP16>, weight[r], x.x);
-          if (t == 2 * j + 1) x.y = fmaf(-kProbScale<FP16>, weight[r], x.y);
-          acc[2 * j] += x.x;
-          acc[2 * j + 1] += x.y;
-          w[j] = pack2<FP16>(x.x, x.y);
+      for (int j = 0; j < 4; ++j) {
+        float2 x = unpack2<FP16>(word[j]);
+        const float2 y = unpack2<FP16>(lw[j]);
+        const float h0 = t == 2 * j ? kProbScale<FP16> * w : 0.f, h1 = t == 2 * j + 1 ? kProbScale<FP16> * w : 0.f;
+        if (bias_partial && w != 0.f) {
+          acc[2 * j] += (x.x + y.x) * f - h0;
+          acc[2 * j + 1] += (x.y + y.y) * f - h1;
         }
+        word[j] = pack2<FP16>(fmaf(x.x, f, -h0), fmaf(x.y, f, -h1));
       }
-      *at = p;
+      return w != 0.f ? p : make_uint4(0u, 0u, 0u, 0u);
+    };
+    int r = part;
+    for (; r + 6 < n_rows; r += 8) {  // four rows at once: their loads are under way together
+      uint4 p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const uint4*>(column + (r + 2 * i) * ld_e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(column + (r + 2 * i) * ld_e) = one(r + 2 * i, p[i]);
     }
+    for (; r < n_rows; r += 2) *reinterpret_cast<uint4*>(column + r * ld_e) = one(r, *reinterpret_cast<const uint4*>(column + r * ld_e));
   }
   if (bias_partial) {
     if (part == 1) {
@@ -704,6 +776,11 @@ int reduction_splits(long long M, long long N, long long K) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// Rows per block of the rescaling pass: 32, or 8 where that would leave half of the machine without blocks.
+int rescale_rows(long long rows, long long vocab) {
+  return ((rows + 31) / 32) * ((vocab + 1023) / 1024) >= 4ll * sm_count() ? 32 : 8;
+}
+
 struct Carve {  // 256-byte aligned pieces of the workspace
   uint8_t* base;
   size_t used;
@@ -722,6 +799,7 @@ struct Buffers {
   float2* norm;
   float* loss;
   unsigned short* e;
+  unsigned short* e_low;  // with a bias gradient: it sums e itself, in 32 bits
   unsigned short* h_copy;
   float* bias_partial;
   float* partial;  // split products of dh or dw
@@ -738,8 +816,14 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
   if (grad) {
     b.norm = c.take<float2>(chunk);
     b.e = c.take<unsigned short>((size_t)chunk * up(vocab, 64));
+    b.e_low = with_bias ? c.take<unsigned short>((size_t)chunk * up(vocab, 64)) : nullptr;
     b.h_copy = c.take<unsigned short>((size_t)chunk * up(hidden, 8));
-    b.bias_partial = with_bias ? c.take<float>((size_t)((chunk + 127) / 128) * vocab) : nullptr;
+    size_t sums = 0;  // of either chunk length
+    for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
+      const size_t n = (size_t)((r + rescale_rows(r, vocab) - 1) / rescale_rows(r, vocab));
+      if (n > sums) sums = n;
+    }
+    b.bias_partial = with_bias ? c.take<float>(sums * vocab) : nullptr;
     size_t part = 0;
     for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
       const int sh = reduction_splits(r, hidden, vocab), sw = reduction_splits(vocab, hidden, r);
@@ -792,6 +876,9 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
   a.N = x.vocab;
   a.k_blocks = (int)((x.hidden + BK - 1) / BK);
   a.splits = 1;
+  // a tensor-core accumulator truncates when it adds, a bias that grows with the number of additions: 1,024 hidden
+  // features per accumulator, joined with rounding (error of the mean loss at 16,384 x 4,096 x 131,072: see kChunkBlocks)
+  a.chunks = (a.k_blocks + kChunkBlocks - 1) / kChunkBlocks;
   a.m_fast = 1;  // the weight streams past, the hidden states stay in L2
   a.group = resident_group(2ll * TM * x.hidden);
   a.error_flag = x.error_flag;
@@ -801,6 +888,7 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
   a.ld_stats = ld_stats;
   a.label_logit = b.label_logit;
   a.e = MODE == kProb ? b.e : nullptr;
+  a.e_low = MODE == kProb ? b.e_low : nullptr;
   a.ld_e = up(x.vocab, 64);
   return launch_product<MODE, false, false, FP16>(map_a, map_b, a, x.stream);
 }
@@ -822,7 +910,7 @@ int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long lo
   a.scale = scale;
   a.ld_out = N;
   a.ld32 = up(N, 4);
-  a.vec16 = N % 8 == 0 && aligned16(out);
+  a.vec16 = N % 16 == 0 && ((uintptr_t)out & 31u) == 0;
   if (sum) {
     a.out32 = sum;
     a.add32 = !first;
@@ -853,10 +941,11 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     if (int rc = xent_finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, b.loss + r0, x.stream))
       return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
-    const int column_blocks = (int)((x.vocab + 1023) / 1024), row_blocks = (int)((n + 127) / 128);
+    const int column_blocks = (int)((x.vocab + 1023) / 1024), block_rows = rescale_rows(n, x.vocab);
+    const int row_blocks = (int)((n + block_rows - 1) / block_rows);
     xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (dw ? 1 : 0))), 256, 0, x.stream>>>(
-        b.e, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
-        reduction == EVOX_REDUCE_NONE, b.scalars, n, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, b.h_copy, ld_copy,
+        b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
+        reduction == EVOX_REDUCE_NONE, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, b.h_copy, ld_copy,
         column_blocks);
     EVOX_LAUNCH_CHECK();
     if (db) {

@@ -104,6 +104,7 @@ struct GemmArgs {
   const long long* labels;  // [batch]
   float2* stats;            // [column slice][M]: (maximum, sum of exponentials)
   float* label_logit;       // [M]
+  long long m_group;        // tiles of rows that are walked before the next tile of columns
 };
 
 // kind::f16 instruction descriptor: D = fp32, A = B = bf16, both K-major, N = 256, M = 128
@@ -165,6 +166,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long n_tiles_n = EPI == 3 ? (a.N + BN - 1) / BN : a.N / BN;
   const long long n_tiles = (a.M / TM) * n_tiles_n;
+  // Layers walk the columns first: their weight stays in the L2 cache. A vocabulary head's weight does not fit, so it streams
+  // past while `m_group` tiles of rows, whose activations do fit, are walked first.
+  auto tile_m = [&](long long tile) {
+    if constexpr (EPI != 3) return tile / n_tiles_n;
+    const long long first = tile / (a.m_group * n_tiles_n) * a.m_group;
+    return first + (tile - first * n_tiles_n) % min(a.m_group, a.M / TM - first);
+  };
+  auto tile_n = [&](long long tile) {
+    if constexpr (EPI != 3) return tile % n_tiles_n;
+    const long long first = tile / (a.m_group * n_tiles_n) * a.m_group;
+    return (tile - first * n_tiles_n) / min(a.m_group, a.M / TM - first);
+  };
   // a CTA pair walks the tile list together; each CTA owns 128 of the tile's 256 rows
   const uint32_t cta_rank = PAIR ? cluster_rank() : 0u;
   const long long tile_first = PAIR ? (long long)(blockIdx.x >> 1) : (long long)blockIdx.x;
@@ -216,8 +229,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int part = (int)(work / n_tiles);
         const int kb_begin = (part * n_chunks / k_split) * chunk_kb;
         const int kb_end = min(((part + 1) * n_chunks / k_split) * chunk_kb, total_kb);
-        const int m0 = (int)((tile / n_tiles_n) * TM) + (int)cta_rank * BM;
-        const int n0 = (int)((tile % n_tiles_n) * BN) + (PAIR ? (int)cta_rank * (BN / 2) : 0);
+        const int m0 = (int)(tile_m(tile) * TM) + (int)cta_rank * BM;
+        const int n0 = (int)(tile_n(tile) * BN) + (PAIR ? (int)cta_rank * (BN / 2) : 0);
         for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) {
             ok = false;
@@ -334,8 +347,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const long long tile = work % n_tiles;
       const int part = (int)(work / n_tiles);
       const int ch0 = part * n_chunks / k_split, ch1 = (part + 1) * n_chunks / k_split;
-      const long long m0 = (tile / n_tiles_n) * TM + (long long)cta_rank * BM;
-      const int n_blk = (int)(tile % n_tiles_n);
+      const long long m0 = tile_m(tile) * TM + (long long)cta_rank * BM;
+      const int n_blk = (int)tile_n(tile);
       const long long n0 = (long long)n_blk * BN;
       if constexpr (ACCUM) {
         // plain product summed over the work item's chunks in registers (one row, 128 columns per thread)
@@ -1031,6 +1044,8 @@ extern "C" int evox_lora_cross_entropy_bf16(const void* h, const void* w, const 
   a.k_split = 1;
   a.operand_format = kFormatBf16;
   a.labels = (const long long*)labels;
+  a.m_group = (48ll << 20) / (2ll * 2 * BM * k);  // 48 MB of activations
+  if (a.m_group < 1) a.m_group = 1;
   a.stats = reinterpret_cast<float2*>(workspace);
   a.label_logit = reinterpret_cast<float*>(a.stats + a.M * ((vocab + kSlice - 1) / kSlice));
   EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));

@@ -68,8 +68,8 @@ class Formula:
         self.dh, self.dw, self.db = G @ w, G.t() @ hv, G.sum(dim=0)
         self.dh_tol = err @ w.abs() + (vocab / 16 + 8) * 2.0**-23 * (size @ w.abs()) + u * self.dh.abs() + tiny
         self.dw_tol = err.t() @ hv.abs() + (rows / 16 + 8) * 2.0**-23 * (size.t() @ hv.abs()) + u * self.dw.abs() + tiny
-        # the bias gradient sums g before its second rounding, in 32 bits
-        self.db_tol = err.sum(dim=0) + (rows + 8) * 2.0**-23 * size.sum(dim=0) + 1e-38
+        # the bias gradient sums 32-bit values: the exponentials with what their rounding left (off by u u)
+        self.db_tol = (size * (rel - 2 * u * (1 + u) + u * u)).sum(dim=0) + (rows + 8) * 2.0**-23 * size.sum(dim=0) + 2.0**-60
 
 
 def near(got, want, tol, what):
