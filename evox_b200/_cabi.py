@@ -107,7 +107,8 @@ def ptr(t: torch.Tensor | None, dtype: torch.dtype | None = None, name: str = "t
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def host_floats(values) -> ctypes.Array:

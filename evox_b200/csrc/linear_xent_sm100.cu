@@ -467,21 +467,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// What a row counts for. valid: its label is not ignore_index. `scalars`: [0] scale of the gradient (its weights are
-// stored as fractions of the largest one, so that any upstream gradient fits the 16-bit type), [1] its inverse,
-// [2] factor of the summed loss. One block: a fixed order, and the counts are whole numbers.
-__global__ void __launch_bounds__(1024)
-    xent_weights_kernel(const long long* __restrict__ labels, long long ignore_index, long long rows, int reduction,
-                        const float* __restrict__ grad_loss, float prob_scale, float* __restrict__ scalars) {
+// What the rows count for, by one block of 1,024 threads (a fixed order, and the counts are whole numbers). `scalars`: [0]
+// scale of the gradient (the rows' weights are stored as fractions of the largest one, so that any upstream gradient
+// fits the 16-bit type), [1] the weights' inverse scale, [2] factor of the summed loss.
+struct Weights {
+  const long long* labels;  // of all rows
+  long long rows;
+  int reduction;
+  const float* grad_loss;
+  float prob_scale;
+  float* scalars;           // null: not wanted
+};
+__device__ void row_weights(const Weights& a, long long ignore_index) {
   __shared__ unsigned long long count_part[32];
   __shared__ float max_part[32];
   unsigned long long count = 0;
   float top = 0.f;
-  for (long long i = threadIdx.x; i < rows; i += 1024) {
-    const bool valid = labels[i] != ignore_index;
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < a.rows; i += 1024) {
+    const bool valid = a.labels[i] != ignore_index;
     count += valid;
-    if (reduction == EVOX_REDUCE_NONE && grad_loss && valid) {
-      const float g = fabsf(grad_loss[i]);
+    if (a.reduction == EVOX_REDUCE_NONE && a.grad_loss && valid) {
+      const float g = fabsf(a.grad_loss[i]);
       if (g <= 3.0e38f) top = fmaxf(top, g);
     }
   }
@@ -500,15 +507,15 @@ __global__ void __launch_bounds__(1024)
       count += count_part[w];
       top = fmaxf(top, max_part[w]);
     }
-    const float per_row = reduction == EVOX_REDUCE_MEAN ? 1.0f / (float)count : 1.0f;  // no valid row: the mean is 0 / 0
+    const float per_row = a.reduction == EVOX_REDUCE_MEAN ? 1.0f / (float)count : 1.0f;  // no valid row: the mean is 0 / 0
     float scale;
-    if (reduction == EVOX_REDUCE_NONE)
-      scale = grad_loss ? (top > 1.0e-36f ? top : 1.0f) : 1.0f;
+    if (a.reduction == EVOX_REDUCE_NONE)
+      scale = a.grad_loss ? (top > 1.0e-36f ? top : 1.0f) : 1.0f;
     else
-      scale = count == 0 ? 0.f : per_row * (grad_loss ? grad_loss[0] : 1.0f);
-    scalars[0] = scale / prob_scale;
-    scalars[1] = 1.0f / scale;
-    scalars[2] = per_row;
+      scale = count == 0 ? 0.f : per_row * (a.grad_loss ? a.grad_loss[0] : 1.0f);
+    a.scalars[0] = scale / a.prob_scale;
+    a.scalars[1] = 1.0f / scale;
+    a.scalars[2] = per_row;
   }
 }
 
@@ -518,7 +525,11 @@ __global__ void __launch_bounds__(1024)
 __global__ void __launch_bounds__(1024)
     xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
                        const long long* __restrict__ labels, long long label_period, long long ignore_index, long long rows, long long vocab,
-                       float2* __restrict__ norm, float* __restrict__ loss) {
+                       float2* __restrict__ norm, float* __restrict__ loss, const Weights weights) {
+  if (weights.scalars && blockIdx.x == gridDim.x - 1) {  // one block more than the rows need
+    row_weights(weights, ignore_index);
+    return;
+  }
   __shared__ float sm[32][33], ss[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = (long long)blockIdx.x * 32 + lane;
@@ -546,10 +557,27 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// One block of 256 threads: out = scalars[2] * the sum of the losses, in 64 bits and a fixed order.
+__device__ void sum_losses(const float* __restrict__ loss, long long rows, const float* __restrict__ scalars, float* __restrict__ out) {
+  __shared__ double part[8];
+  double s = 0.0;
+#pragma unroll 8
+  for (long long i = threadIdx.x; i < rows; i += 256) s += (double)loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) s += part[w];
+    out[0] = (float)(s * (double)scalars[2]);
+  }
+}
+
 // e -> g in place (see the head of the file), `block_rows` (at most 32) rows x 1,024 columns per block, eight columns per
 // thread; column sums of the block's rows for the bias gradient, which is a 32-bit result: they take e with what its
-// rounding left. The blocks of the last grid row copy the hidden states for the weight gradient, with zeros where the
-// label is ignored: 0 x inf in a padded row must not reach dw.
+// rounding left. The blocks of one more grid row copy the hidden states for the weight gradient, with zeros where the
+// label is ignored: 0 x inf in a padded row must not reach dw. The first block of another one sums the losses of
+// all rows once they are there.
 template <bool FP16>
 __global__ void __launch_bounds__(256)
     xent_rescale_kernel(unsigned short* __restrict__ e, const unsigned short* __restrict__ e_low, long long ld_e,
@@ -557,11 +585,17 @@ __global__ void __launch_bounds__(256)
                         const long long* __restrict__ labels, long long ignore_index, const float* __restrict__ grad_loss, int per_row,
                         const float* __restrict__ scalars, long long rows, int block_rows, long long vocab,
                         float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h, long long hidden,
-                        unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks) {
+                        unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks, const float* __restrict__ loss, long long all_rows,
+                        float* __restrict__ loss_out) {
+  if ((int)blockIdx.y > column_blocks) {
+    if (blockIdx.x == 0 && loss_out) sum_losses(loss, all_rows, scalars, loss_out);
+    return;
+  }
   const long long row0 = (long long)blockIdx.x * block_rows;
   const int n_rows = (int)min((long long)block_rows, rows - row0);
   const int tid = threadIdx.x;
-  if ((int)blockIdx.y >= column_blocks) {
+  if ((int)blockIdx.y == column_blocks) {
+    if (!h_out) return;
     const int pieces = (int)(ld_h_out / 8);
     for (int r = 0; r < n_rows; ++r) {
       const bool keep = labels[row0 + r] != ignore_index;
@@ -662,52 +696,62 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// db[v] (+)= scale * sum over the row blocks, in their order.
-__global__ void __launch_bounds__(256)
-    xent_bias_kernel(const float* __restrict__ partial, int blocks, long long vocab, const float* __restrict__ scalars, int add,
-                     float* __restrict__ db) {
-  const long long v = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (v >= vocab) return;
-  float s = 0.f;
-  for (int b = 0; b < blocks; ++b) s += partial[(long long)b * vocab + v];
-  s *= scalars[0];
-  db[v] = add ? db[v] + s : s;
-}
-
-// out[r][c] = sum over the splits, in their order, of partial[split][r][c] (partials are scaled already).
+// The end of a gradient: up to two products whose reduction was divided (sum over the splits, in their order, of partial
+// results that are scaled already) and the bias gradient (scale times the sum over the row blocks, in their order; added to
+// what the earlier row chunks left). Blocks are dealt to the three in turn.
+struct Join {
+  const float* partial;  // [splits][rows][ld32]
+  unsigned short* out;   // [rows][cols], 16 bits
+  long long rows, cols, ld32;
+  int splits, blocks;    // blocks: 0 if there is nothing to join
+};
+struct BiasSum {
+  const float* partial;  // [row_blocks][vocab]
+  float* out;
+  const float* scale;
+  long long vocab;
+  int row_blocks, add, blocks;
+};
 template <bool FP16>
-__global__ void __launch_bounds__(256)
-    xent_join_kernel(const float* __restrict__ partial, int splits, long long rows, long long cols, long long ld32,
-                     unsigned short* __restrict__ out, long long ld_out) {
-  const long long quads = (cols + 3) / 4, n = rows * quads;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+__global__ void __launch_bounds__(256) xent_join_kernel(const Join dh, const Join dw, const BiasSum db) {
+  int block = blockIdx.x;
+  if (block < db.blocks) {
+    const long long v = (long long)block * 256 + threadIdx.x;
+    if (v >= db.vocab) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int b = 0; b < db.row_blocks; ++b) s += __ldg(db.partial + (long long)b * db.vocab + v);
+    s *= db.scale[0];
+    db.out[v] = db.add ? db.out[v] + s : s;
+    return;
+  }
+  block -= db.blocks;
+  const Join a = block < dh.blocks ? dh : dw;
+  if (block >= dh.blocks) block -= dh.blocks;
+  const long long quads = (a.cols + 3) / 4, n = a.rows * quads;
+  for (long long i = (long long)block * 256 + threadIdx.x; i < n; i += (long long)a.blocks * 256) {
     const long long r = i / quads, c = (i - r * quads) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < splits; ++k) {
-      const float4 p = *reinterpret_cast<const float4*>(partial + ((long long)k * rows + r) * ld32 + c);
+#pragma unroll 4
+    for (int k = 0; k < a.splits; ++k) {
+      const float4 p = __ldcs(reinterpret_cast<const float4*>(a.partial + ((long long)k * a.rows + r) * a.ld32 + c));
       s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
     }
-    const float v[4] = {s.x, s.y, s.z, s.w};
+    unsigned short* to = a.out + r * a.cols + c;
+    if (a.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack2<FP16>(s.x, s.y), pack2<FP16>(s.z, s.w));
+    } else {
+      const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < cols) out[r * ld_out + c + j] = pack1<FP16>(v[j]);
+      for (int j = 0; j < 4; ++j)
+        if (c + j < a.cols) to[j] = pack1<FP16>(v[j]);
+    }
   }
 }
 
 // Sum of the rows' losses times the reduction's factor: one block, 64-bit sums in a fixed order.
-__global__ void __launch_bounds__(1024)
-    xent_loss_sum_kernel(const float* __restrict__ loss, long long rows, const float* __restrict__ scalars, float* __restrict__ out) {
-  __shared__ double part[32];
-  double s = 0.0;
-  for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)loss[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) s += part[w];
-    out[0] = (float)(s * (double)scalars[2]);
-  }
+__global__ void __launch_bounds__(256) xent_loss_sum_kernel(const float* __restrict__ loss, long long rows, const float* __restrict__ scalars, float* __restrict__ out) {
+  sum_losses(loss, rows, scalars, out);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -802,8 +846,9 @@ struct Buffers {
   unsigned short* e_low;  // with a bias gradient: it sums e itself, in 32 bits
   unsigned short* h_copy;
   float* bias_partial;
-  float* partial;  // split products of dh or dw
-  float* dw_sum;   // running dw over the row chunks
+  float* partial_dh;  // products whose reduction is divided
+  float* partial_dw;
+  float* dw_sum;      // running dw over the row chunks
 };
 
 size_t layout(Buffers& b, void* base, long long rows, long long hidden, long long vocab, long long chunk, bool grad, bool with_bias) {
@@ -824,13 +869,14 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
       if (n > sums) sums = n;
     }
     b.bias_partial = with_bias ? c.take<float>(sums * vocab) : nullptr;
-    size_t part = 0;
+    size_t part_dh = 0;
     for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
-      const int sh = reduction_splits(r, hidden, vocab), sw = reduction_splits(vocab, hidden, r);
-      if (sh > 1 && part < (size_t)sh * r * up(hidden, 4)) part = (size_t)sh * r * up(hidden, 4);
-      if (sw > 1 && part < (size_t)sw * vocab * up(hidden, 4)) part = (size_t)sw * vocab * up(hidden, 4);
+      const int splits = reduction_splits(r, hidden, vocab);
+      if (splits > 1 && part_dh < (size_t)splits * r * up(hidden, 4)) part_dh = (size_t)splits * r * up(hidden, 4);
     }
-    b.partial = part ? c.take<float>(part) : nullptr;
+    const int splits_dw = chunk < rows ? 1 : reduction_splits(vocab, hidden, rows);
+    b.partial_dh = part_dh ? c.take<float>(part_dh) : nullptr;
+    b.partial_dw = splits_dw > 1 ? c.take<float>((size_t)splits_dw * vocab * up(hidden, 4)) : nullptr;
     b.dw_sum = chunk < rows ? c.take<float>((size_t)vocab * up(hidden, 4)) : nullptr;
   }
   return c.used;
@@ -863,6 +909,15 @@ struct Head {
   int* error_flag;
   cudaStream_t stream;
 };
+
+int finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
+           long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const Weights& weights, cudaStream_t stream) {
+  const int slices = (int)((vocab + kSlice - 1) / kSlice);
+  xent_finish_kernel<<<(unsigned)((rows + 31) / 32 + (weights.scalars ? 1 : 0)), 1024, 0, stream>>>(
+      stats, ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, weights);
+  EVOX_LAUNCH_CHECK();
+  return EVOX_OK;
+}
 
 // Logits of `n` rows from `r0` on: (maximum, sum) per slice, the labels' logits, and with MODE == kProb the exponentials.
 template <int MODE, bool FP16>
@@ -897,7 +952,7 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
 // `sum`: running 32-bit sum over row chunks (null: this product is the whole); `first`, `last`: which chunk.
 template <bool A_MN, bool FP16>
 int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long long M, long long N, long long K, int m_fast, int group,
-                     void* out, const float* scale, float* partial, float* sum, bool first, bool last, int* error_flag,
+                     void* out, const float* scale, float* partial, float* sum, bool first, bool last, Join* join, int* error_flag,
                      cudaStream_t stream) {
   ProductArgs a = {};
   a.M = M;
@@ -922,51 +977,57 @@ int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long lo
   }
   if (int rc = launch_product<kOut, A_MN, true, FP16>(map_a, map_b, a, stream)) return rc;
   if (a.splits > 1) {
-    const long long n = M * ((N + 3) / 4), blocks = (n + 255) / 256, cap = 16ll * sm_count();
-    xent_join_kernel<FP16><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(partial, a.splits, M, N, a.ld32,
-                                                                                    reinterpret_cast<unsigned short*>(out), N);
-    EVOX_LAUNCH_CHECK();
+    const long long blocks = (M * ((N + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
+    *join = Join{partial, reinterpret_cast<unsigned short*>(out), M, N, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
   }
   return EVOX_OK;
 }
 
 template <bool FP16>
-int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reduction, const float* grad_loss, void* dh, void* dw, float* db) {
+int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reduction, const float* grad_loss, float* loss, void* dh, void* dw,
+                  float* db) {
   const int slices = (int)((x.vocab + kSlice - 1) / kSlice);
   const long long ld_e = up(x.vocab, 64), ld_copy = up(x.hidden, 8);
+  const bool per_row = reduction == EVOX_REDUCE_NONE;
+  float* row_loss = per_row ? loss : b.loss;
   for (long long r0 = 0; r0 < x.rows; r0 += chunk) {
     const long long n = x.rows - r0 < chunk ? x.rows - r0 : chunk;
     const bool first = r0 == 0, last = r0 + n == x.rows;
     if (int rc = logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
-    if (int rc = xent_finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, b.loss + r0, x.stream))
+    const Weights weights = {x.labels, x.rows, reduction, grad_loss, kProbScale<FP16>, first ? b.scalars : nullptr};
+    if (int rc = finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, row_loss + r0, weights, x.stream))
       return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
     const int column_blocks = (int)((x.vocab + 1023) / 1024), block_rows = rescale_rows(n, x.vocab);
     const int row_blocks = (int)((n + block_rows - 1) / block_rows);
-    xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (dw ? 1 : 0))), 256, 0, x.stream>>>(
-        b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss ? grad_loss + r0 * (reduction == EVOX_REDUCE_NONE) : nullptr,
-        reduction == EVOX_REDUCE_NONE, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, b.h_copy, ld_copy,
-        column_blocks);
+    const bool sum_here = last && !per_row;
+    xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (sum_here ? 2 : dw ? 1 : 0))), 256, 0, x.stream>>>(
+        b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss && per_row ? grad_loss + r0 : nullptr,
+        per_row, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, dw ? b.h_copy : nullptr, ld_copy,
+        column_blocks, row_loss, x.rows, sum_here ? loss : nullptr);
     EVOX_LAUNCH_CHECK();
-    if (db) {
-      xent_bias_kernel<<<(unsigned)((x.vocab + 255) / 256), 256, 0, x.stream>>>(b.bias_partial, row_blocks, x.vocab, b.scalars, !first, db);
-      EVOX_LAUNCH_CHECK();
-    }
+    Join join_dh = {}, join_dw = {};
     CUtensorMap map_a, map_b;
     if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
       if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 128, FP16)) return rc;
       if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
       unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;
-      if (int rc = gradient_product<false, FP16>(map_a, map_b, n, x.hidden, x.vocab, 0, 8, out, b.scalars, b.partial, nullptr, true, true,
-                                                 x.error_flag, x.stream))
+      if (int rc = gradient_product<false, FP16>(map_a, map_b, n, x.hidden, x.vocab, 0, 8, out, b.scalars, b.partial_dh, nullptr, true, true,
+                                                 &join_dh, x.error_flag, x.stream))
         return rc;
     }
     if (dw) {  // g^T (contiguous along vocab) times the hidden states (contiguous along hidden)
       if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 64, FP16)) return rc;
       if (int rc = map_16(&map_b, b.h_copy, x.hidden, n, ld_copy, 64, FP16)) return rc;
       if (int rc = gradient_product<true, FP16>(map_a, map_b, x.vocab, x.hidden, n, 0, resident_group(2ll * TN * n), dw, b.scalars,
-                                                b.partial, b.dw_sum, first, last, x.error_flag, x.stream))
+                                                b.partial_dw, b.dw_sum, first, last, &join_dw, x.error_flag, x.stream))
         return rc;
+    }
+    BiasSum bias = {};
+    if (db) bias = BiasSum{b.bias_partial, db, b.scalars, x.vocab, row_blocks, !first, (int)((x.vocab + 255) / 256)};
+    if (const int blocks = join_dh.blocks + join_dw.blocks + bias.blocks) {
+      xent_join_kernel<FP16><<<(unsigned)blocks, 256, 0, x.stream>>>(join_dh, join_dw, bias);
+      EVOX_LAUNCH_CHECK();
     }
   }
   return EVOX_OK;
@@ -976,11 +1037,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
 
 int xent_finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
                 long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, cudaStream_t stream) {
-  const int slices = (int)((vocab + kSlice - 1) / kSlice);
-  xent_finish_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, stream>>>(stats, ld_stats, slices, label_logit, labels, label_period,
-                                                                      ignore_index, rows, vocab, norm, loss);
-  EVOX_LAUNCH_CHECK();
-  return EVOX_OK;
+  return finish(stats, ld_stats, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, Weights{}, stream);
 }
 
 }  // namespace evox
@@ -1004,14 +1061,12 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
                "linear_cross_entropy: workspace too small");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
-  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
   if (int rc = dtype == EVOX_DTYPE_FP16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
-  float* per_row = reduction == EVOX_REDUCE_NONE ? loss : b.loss;
-  if (int rc = xent_finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, per_row, s)) return rc;
-  if (reduction != EVOX_REDUCE_NONE) {
-    xent_weights_kernel<<<1, 1024, 0, s>>>(x.labels, ignore_index, rows, reduction, nullptr, 1.0f, b.scalars);
-    EVOX_LAUNCH_CHECK();
-    xent_loss_sum_kernel<<<1, 1024, 0, s>>>(b.loss, rows, b.scalars, loss);
+  const bool per_row = reduction == EVOX_REDUCE_NONE;
+  const Weights weights = {x.labels, rows, reduction, nullptr, 1.0f, per_row ? nullptr : b.scalars};
+  if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, per_row ? loss : b.loss, weights, s)) return rc;
+  if (!per_row) {
+    xent_loss_sum_kernel<<<1, 256, 0, s>>>(b.loss, rows, b.scalars, loss);
     EVOX_LAUNCH_CHECK();
   }
   return EVOX_OK;
@@ -1045,17 +1100,6 @@ extern "C" int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const
                "linear_cross_entropy_grad: workspace too small");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
-  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
-  const bool fp16 = dtype == EVOX_DTYPE_FP16;
-  xent_weights_kernel<<<1, 1024, 0, s>>>(x.labels, ignore_index, rows, reduction, grad_loss, fp16 ? kProbScale<true> : kProbScale<false>, b.scalars);
-  EVOX_LAUNCH_CHECK();
-  if (reduction == EVOX_REDUCE_NONE) b.loss = loss;
-  if (int rc = fp16 ? gradient_pass<true>(x, b, chunk, reduction, grad_loss, dh, dw, dbias)
-                    : gradient_pass<false>(x, b, chunk, reduction, grad_loss, dh, dw, dbias))
-    return rc;
-  if (reduction != EVOX_REDUCE_NONE) {
-    xent_loss_sum_kernel<<<1, 1024, 0, s>>>(b.loss, rows, b.scalars, loss);
-    EVOX_LAUNCH_CHECK();
-  }
-  return EVOX_OK;
+  return dtype == EVOX_DTYPE_FP16 ? gradient_pass<true>(x, b, chunk, reduction, grad_loss, loss, dh, dw, dbias)
+                                  : gradient_pass<false>(x, b, chunk, reduction, grad_loss, loss, dh, dw, dbias);
 }

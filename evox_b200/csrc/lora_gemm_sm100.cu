@@ -1048,7 +1048,6 @@ extern "C" int evox_lora_cross_entropy_bf16(const void* h, const void* w, const 
   if (a.m_group < 1) a.m_group = 1;
   a.stats = reinterpret_cast<float2*>(workspace);
   a.label_logit = reinterpret_cast<float*>(a.stats + a.M * ((vocab + kSlice - 1) / kSlice));
-  EVOX_CUDA(cudaMemsetAsync(error_flag, 0, sizeof(int32_t), s));
   if (int rc = launch_gemm(h, a.M, w, vocab, k, a, false, s)) return rc;
   return xent_finish(a.stats, a.M, a.label_logit, a.labels, batch, ignore_index, a.M, vocab, nullptr, loss, s);
 }

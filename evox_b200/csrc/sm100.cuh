@@ -160,6 +160,12 @@ inline int encode_fn(EncodeTiledFn* out) {
     EVOX_REQUIRE(p != nullptr && q == cudaDriverEntryPointSuccess, EVOX_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     fn = reinterpret_cast<EncodeTiledFn>(p);
   }
+  // the encoder is a driver call: a thread that made no runtime call yet (one of autograd's) has no context to make it in
+  static thread_local bool bound = false;
+  if (!bound) {
+    EVOX_CUDA(cudaFree(nullptr));
+    bound = true;
+  }
   *out = fn;
   return EVOX_OK;
 }

@@ -2,8 +2,8 @@
 
 from __future__ import annotations
 
+from array import array
 from collections.abc import Iterable
-from ctypes import c_int32, c_int64, c_uint64
 from operator import attrgetter
 
 import torch
@@ -22,10 +22,10 @@ def _norm(tensors: torch.Tensor | Iterable[torch.Tensor], max_norm: float, clip:
     if n == 0:
         raise err("the list of gradients is empty")
     # whole-list passes instead of a loop with several calls per tensor: a list of hundreds costs tens of microseconds
-    types = list(map(attrgetter("dtype"), tensors))
+    types = set(map(attrgetter("dtype"), tensors))
     devices = set(map(torch.Tensor.get_device, tensors))
-    if not set(types) <= _DTYPES.keys():
-        raise err(f"gradients must be bfloat16, float16 or float32, got {sorted(map(str, set(types) - _DTYPES.keys()))}")
+    if not types <= _DTYPES.keys():
+        raise err(f"gradients must be bfloat16, float16 or float32, got {sorted(map(str, types - _DTYPES.keys()))}")
     if len(devices) != 1 or -1 in devices:
         raise err(f"gradients must live on one CUDA device (evox_b200 has no CPU path), got {sorted({str(t.device) for t in tensors})}")
     if devices != {torch.cuda.current_device()}:
@@ -36,10 +36,10 @@ def _norm(tensors: torch.Tensor | Iterable[torch.Tensor], max_norm: float, clip:
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nbytes = _cabi.lib.evox_grad_norm_workspace_bytes(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _cabi.check(_cabi.lib.evox_clip_grad_norm(
-        (c_uint64 * n)(*map(torch.Tensor.data_ptr, tensors)), (c_int64 * n)(*map(torch.Tensor.numel, tensors)),
-        (c_int32 * n)(*map(_DTYPES.__getitem__, types)), n, max_norm, int(clip), norm.data_ptr(), ws.data_ptr(), nbytes,
-        _cabi.stream_ptr(dev)))
+    table = (array("Q", map(torch.Tensor.data_ptr, tensors)), array("q", map(torch.Tensor.numel, tensors)),
+             array("i", [_DTYPES[types.pop()]]) * n if len(types) == 1 else array("i", [_DTYPES[t.dtype] for t in tensors]))
+    _cabi.check(_cabi.lib.evox_clip_grad_norm(*(a.buffer_info()[0] for a in table), n, max_norm, int(clip), norm.data_ptr(), ws.data_ptr(),
+                                              nbytes, _cabi.stream_ptr(dev)))
     return norm
 
 

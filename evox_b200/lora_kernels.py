@@ -29,6 +29,13 @@ _pending_flags: list[tuple[str, torch.Tensor]] = []
 def raise_on_kernel_errors() -> None:
     """Synchronise on and check every tensor-core launch since the last call; raise if a bounded
     device-side wait expired (1 producer, 2 / 3 issuer, 4 epilogue) or shared memory was misaligned (5)."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        return  # nothing can be read back now
+    for index, word in _status_words.items():
+        code = int(word)
+        if code != 0:
+            word.zero_()
+            raise _cabi.EvoxKernelError(f"a tensor-core kernel on cuda:{index} gave up with status {code} (a bounded wait expired)")
     pending, _pending_flags[:] = list(_pending_flags), []
     for what, flag in pending:
         code = int(flag)
@@ -36,13 +43,19 @@ def raise_on_kernel_errors() -> None:
             raise _cabi.EvoxKernelError(f"{what}: the tensor-core kernel gave up with status {code} (a bounded wait expired)")
 
 
-def kernel_flag(what: str, dev: torch.device) -> torch.Tensor:
-    """A status word for one tensor-core launch that sets it itself, remembered for `raise_on_kernel_errors`."""
-    err = torch.empty(1, dtype=torch.int32, device=dev)
-    if not torch.cuda.is_current_stream_capturing():  # a captured launch's flag belongs to the graph's replays
-        _pending_flags.append((what, err))
-        del _pending_flags[:-256]
-    return err
+# One status word per device for the launches that share theirs: a kernel writes it only when a wait expires, and the
+# launches after that give up as well until `raise_on_kernel_errors` has reported it.
+_status_words: dict[int, torch.Tensor] = {}
+
+
+def status_word(dev: torch.device) -> torch.Tensor:
+    word = _status_words.get(dev.index)
+    if word is None:
+        word = torch.zeros(1, dtype=torch.int32, device=dev)
+        if not torch.cuda.is_current_stream_capturing():  # a word of a graph's own is set to 0 by its replays only
+            torch.cuda.current_stream(dev).synchronize()  # once: launches on other streams may use it next
+            _status_words[dev.index] = word
+    return word
 
 
 def _seeds(seeds: torch.Tensor) -> torch.Tensor:
@@ -238,7 +251,7 @@ def lora_layer_cross_entropy(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tens
     loss = torch.empty(pop, batch, dtype=torch.float32, device=dev)
     nbytes = lib.evox_lora_cross_entropy_workspace_bytes(pop, batch, vocab)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = kernel_flag("lora_layer_cross_entropy", dev)
+    err = status_word(dev)
     _cabi.check(
         lib.evox_lora_cross_entropy_bf16(
             _cabi.ptr(h), _cabi.ptr(w), _cabi.ptr(bias_f), _cabi.ptr(t), _cabi.ptr(seeds), counter + _ceil4(rank * k),

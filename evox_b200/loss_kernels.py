@@ -12,7 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _cabi
-from .lora_kernels import kernel_flag
+from .lora_kernels import status_word
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_grad"]
 
@@ -20,47 +20,58 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
-def _operand(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+def _operand(x: torch.Tensor, rows: int, hidden: int) -> tuple[torch.Tensor, int]:
     """`x` (rows, hidden) with rows that start on 16-byte boundaries, and its row stride; a view is used as it is
     where it can be, anything else is copied."""
-    rows, hidden = x.shape
-    stride = x.stride(0) if rows > 1 else (hidden + 7) // 8 * 8
-    if x.stride(1) == 1 and stride >= hidden and stride % 8 == 0 and x.data_ptr() % 16 == 0:
+    stride, step = x.stride()
+    if rows == 1:
+        stride = (hidden + 7) // 8 * 8
+    if (step == 1 or hidden == 1) and stride % 8 == 0 and stride >= hidden and x.data_ptr() % 16 == 0:
         return x, stride
     pad = -hidden % 8
-    x = F.pad(x, (0, pad)) if pad else x.contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone()
+    with torch.no_grad():
+        x = F.pad(x, (0, pad)) if pad else x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
     return x, hidden + pad
 
 
-def _arguments(h, weight, labels, bias, reduction):
-    """Checked and flattened arguments: (h, weight, labels, bias fp32, leading shape)."""
+def _refuse(h, weight, labels, bias, reduction):
+    """Say what is wrong with the arguments."""
     err = _cabi.EvoxKernelError
     if reduction not in _REDUCTIONS:
         raise err(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if h.dtype not in _DTYPES or weight.dtype != h.dtype:
         raise err(f"hidden states and weight must both be bfloat16 or both float16, got {h.dtype} and {weight.dtype}")
-    if weight.ndim != 2 or h.ndim < 1 or h.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:
+    if weight.ndim != 2 or h.ndim < 1 or h.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise err(f"shape mismatch: hidden states {tuple(h.shape)}, weight {tuple(weight.shape)}")
     if labels.dtype != torch.int64 or labels.shape != h.shape[:-1]:
         raise err(f"labels must be int64 of shape {tuple(h.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
     if bias is not None and (bias.shape != weight.shape[:1] or not bias.is_floating_point()):
         raise err(f"bias must be floating point of shape ({weight.shape[0]},), got {bias.dtype} {tuple(bias.shape)}")
     for name, t in (("hidden states", h), ("weight", weight), ("labels", labels), ("bias", bias)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise err(f"{name} must live on a CUDA device (evox_b200 has no CPU path), got {t.device}")
-        if t.device != h.device:
-            raise err(f"{name} lives on {t.device}, hidden states on {h.device}")
-    return (h.reshape(-1, h.shape[-1]), weight, labels.reshape(-1).contiguous(),
-            None if bias is None else bias.to(torch.float32).contiguous(), tuple(h.shape[:-1]))
+        if t is not None:
+            _cabi.ptr(t.reshape(-1)[:0], None, name)  # on a CUDA device, and on the current one
 
 
-def _pointer(x: torch.Tensor, name: str) -> int:
-    _cabi.ptr(x[:1, :1] if x.ndim == 2 else x, None, name)  # device checks; the strides were looked at already
-    return x.data_ptr()
+def _arguments(h, weight, labels, bias, reduction):
+    """Checked and flattened arguments: (h, weight, labels, bias fp32, leading shape)."""
+    dtype, shape = h.dtype, h.shape
+    rest = shape[:-1]
+    here = torch.cuda.current_device() if h.is_cuda else -1
+    if (dtype not in _DTYPES or weight.dtype != dtype or weight.ndim != 2 or not shape or weight.shape[1] != shape[-1] or weight.numel() == 0
+            or reduction not in _REDUCTIONS or labels.dtype != torch.int64 or labels.shape != rest
+            or h.get_device() != here or weight.get_device() != here or labels.get_device() != here or here < 0
+            or (bias is not None and (bias.shape != weight.shape[:1] or not bias.is_floating_point() or bias.get_device() != here))):
+        _refuse(h, weight, labels, bias, reduction)
+        raise _cabi.EvoxKernelError("arguments of linear_cross_entropy do not fit together")
+    if len(shape) != 2:
+        h, labels = h.reshape(-1, shape[-1]), labels.reshape(-1)
+    if not labels.is_contiguous():
+        labels = labels.contiguous()
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.detach().to(torch.float32).contiguous()
+    return h, weight, labels, bias, rest
 
 
 def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
@@ -69,40 +80,39 @@ def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
     vocab = weight.shape[0]
     if rows == 0:
         return torch.full(shape if reduction == "none" else (), float("nan") if reduction == "mean" else 0.0, device=dev)
-    (h, ld_h), (weight, ld_w) = _operand(h), _operand(weight)
+    (h, ld_h), (weight, ld_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
     loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
     lib = _cabi.lib
     nbytes = lib.evox_linear_cross_entropy_workspace_bytes(rows, hidden, vocab)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = kernel_flag("linear_cross_entropy", dev)
     _cabi.check(lib.evox_linear_cross_entropy(
-        _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
-        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(loss), _cabi.ptr(ws), nbytes, _cabi.ptr(err),
+        h.data_ptr(), ld_h, weight.data_ptr(), ld_w, _DTYPES[h.dtype], None if bias is None else bias.data_ptr(), labels.data_ptr(),
+        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], loss.data_ptr(), ws.data_ptr(), nbytes, status_word(dev).data_ptr(),
         _cabi.stream_ptr(dev)))
     return loss
 
 
 def _loss_and_grad(h, weight, labels, bias, ignore_index, reduction, shape, grad_loss, chunk_rows, wanted):
     """(loss, dh (rows, hidden), dw, dbias fp32); `wanted`: which of the three gradients are computed."""
-    dev = h.device
+    dev, dtype = h.device, h.dtype
     rows, hidden = h.shape
     vocab = weight.shape[0]
-    dh = torch.empty(rows, hidden, dtype=h.dtype, device=dev) if wanted[0] else None
-    dw = torch.empty(vocab, hidden, dtype=h.dtype, device=dev) if wanted[1] else None
+    dh = torch.empty(rows, hidden, dtype=dtype, device=dev) if wanted[0] else None
+    dw = torch.empty(vocab, hidden, dtype=dtype, device=dev) if wanted[1] else None
     db = torch.empty(vocab, dtype=torch.float32, device=dev) if wanted[2] and bias is not None else None
     if rows == 0:
         return _loss(h, weight, labels, bias, ignore_index, reduction, shape), dh, *(None if g is None else g.zero_() for g in (dw, db))
-    (h, ld_h), (weight, ld_w) = _operand(h), _operand(weight)
+    (h, ld_h), (weight, ld_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
     loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
     lib = _cabi.lib
     chunk = lib.evox_linear_cross_entropy_chunk_rows(rows, vocab) if chunk_rows is None else chunk_rows
     nbytes = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, hidden, vocab, chunk, db is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = kernel_flag("linear_cross_entropy_grad", dev)
     _cabi.check(lib.evox_linear_cross_entropy_grad(
-        _pointer(h, "hidden states"), ld_h, _pointer(weight, "weight"), ld_w, _DTYPES[h.dtype], _cabi.ptr(bias), _cabi.ptr(labels),
-        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], _cabi.ptr(grad_loss), chunk, _cabi.ptr(loss), _cabi.ptr(dh),
-        _cabi.ptr(dw), _cabi.ptr(db), _cabi.ptr(ws), nbytes, _cabi.ptr(err), _cabi.stream_ptr(dev)))
+        h.data_ptr(), ld_h, weight.data_ptr(), ld_w, _DTYPES[dtype], None if bias is None else bias.data_ptr(), labels.data_ptr(),
+        ignore_index, rows, hidden, vocab, _REDUCTIONS[reduction], None if grad_loss is None else grad_loss.data_ptr(), chunk,
+        loss.data_ptr(), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+        ws.data_ptr(), nbytes, status_word(dev).data_ptr(), _cabi.stream_ptr(dev)))
     return loss, dh, dw, db
 
 
@@ -113,7 +123,7 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
     (`dbias` is None without a bias). Arguments as for `linear_cross_entropy`; `grad_loss` is the upstream gradient
     (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
     are held at a time (default: all, up to 2 GiB of them)."""
-    flat, weight, labels, bias_f, shape = _arguments(h.detach(), weight.detach(), labels, None if bias is None else bias.detach(), reduction)
+    flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
     if chunk_rows is not None and chunk_rows < 1:
         raise _cabi.EvoxKernelError(f"chunk_rows must be at least 1, got {chunk_rows}")
     if grad_loss is not None:
@@ -122,7 +132,9 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
             raise _cabi.EvoxKernelError(f"grad_loss must have shape {tuple(want)}, got {tuple(grad_loss.shape)}")
         grad_loss = grad_loss.detach().to(device=flat.device, dtype=torch.float32).contiguous()
     loss, dh, dw, db = _loss_and_grad(flat, weight, labels, bias_f, ignore_index, reduction, shape, grad_loss, chunk_rows, (True, True, True))
-    return loss, dh.view(h.shape), dw, None if bias is None else db.to(bias.dtype)
+    if bias is not None and bias.dtype != torch.float32:
+        db = db.to(bias.dtype)
+    return loss, dh if dh.shape == h.shape else dh.view(h.shape), dw, db
 
 
 class _LinearCrossEntropy(torch.autograd.Function):

@@ -581,7 +581,8 @@ int evox_bench_compare_rate(const float* in, uint32_t* out, int32_t iterations, 
  * 16-byte aligned bases; bias (vocab, fp32) or NULL; fp32 sums. A row whose label is ignore_index has
  * loss 0; any other label outside [0, vocab) gives NaN. loss: rows values (EVOX_REDUCE_NONE) or one.
  * The logits are not stored: the workspace holds 8 bytes per row and 128 columns. error_flag: a
- * device int32, set to 0 by the call and to a status if a bounded device-side wait expired. */
+ * device int32 that holds 0, set to a status if a bounded device-side wait expired; one word may serve
+ * any number of calls. */
 size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
 int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype,
                               const float* bias, const int64_t* labels, int64_t ignore_index,

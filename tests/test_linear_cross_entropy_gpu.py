@@ -378,9 +378,15 @@ def test_backward_in_a_graph(cuda):
 
 
 @gpu
-def test_no_wait_expired(cuda):
-    from evox_b200.lora_kernels import raise_on_kernel_errors
+def test_no_wait_expired_and_a_status_is_reported_once(cuda):
+    from evox_b200._cabi import EvoxKernelError
+    from evox_b200.lora_kernels import raise_on_kernel_errors, status_word
 
+    raise_on_kernel_errors()
+    assert status_word(cuda) is status_word(torch.device("cuda:0"))
+    status_word(cuda).fill_(4)  # what a kernel whose wait expired would leave
+    with pytest.raises(EvoxKernelError, match="status 4"):
+        raise_on_kernel_errors()
     raise_on_kernel_errors()
 
 
