@@ -50,6 +50,7 @@ struct ProductArgs {
   int splits;              // the reduction is divided among this many work items per tile (kOut)
   int chunks;              // accumulators that a tile's reduction is divided among (kLoss, kProb)
   int tiles_m, tiles_n;
+  uint32_t stage_bytes;    // what the copies of a stage bring to both CTAs
   int m_fast, group;       // tiles run through `group` of the one direction, then all of the other
   uint32_t idesc;
   int* error_flag;
@@ -200,13 +201,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if (cta_rank == 0) mbar_expect_tx(full_bar(s), 2 * kStageBytes);
+          if (cta_rank == 0) mbar_expect_tx(full_bar(s), a.stage_bytes);
           const uint32_t fb = leader_full0 + 8u * s, sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
           const int k0 = kb * BK;
           if constexpr (A_MN) {
             tma_load_2d_pair(sa, &map_a, fb, m0, k0);
             tma_load_2d_pair(sa + kOperandBytes / 2, &map_a, fb, m0 + 64, k0);
-          } else {
+          } else if (cta_rank == 0 || a.stage_bytes == 2 * kStageBytes) {
             tma_load_2d_pair(sa, &map_a, fb, k0, m0);
           }
           if constexpr (B_MN) {
@@ -535,6 +536,7 @@ __global__ void __launch_bounds__(1024)
   const long long row = (long long)blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < rows) {
+#pragma unroll 4
     for (int j = warp; j < slices; j += 32) {
       const float2 p = __ldg(stats + (long long)j * ld_stats + row);
       const float top = fmaxf(m, p.x);
@@ -545,15 +547,19 @@ __global__ void __launch_bounds__(1024)
   sm[warp][lane] = m;
   ss[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && row < rows) {
-    for (int w = 1; w < 32; ++w) m = fmaxf(m, sm[w][lane]);
-    const float base = m == -INFINITY ? 0.f : m;
-    s = 0.f;
-    for (int w = 0; w < 32; ++w) s += ss[w][lane] * expf(sm[w][lane] - base);
-    const long long y = labels[row % label_period];
+  // a warp per row: lanes are the 32 partial results
+  const long long mine = (long long)blockIdx.x * 32 + warp;
+  if (mine >= rows) return;
+  const float pm = sm[lane][warp];
+  m = pm;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  s = warp_sum(ss[lane][warp] * expf(pm - (m == -INFINITY ? 0.f : m)));
+  if (lane == 0) {
+    const long long y = labels[mine % label_period];
     const bool ignored = y == ignore_index, outside = !ignored && (y < 0 || y >= vocab);
-    if (norm) norm[row] = make_float2(m, outside ? NAN : 1.0f / s);
-    loss[row] = ignored ? 0.f : (outside ? NAN : (m - label_logit[row]) + logf(s));
+    if (norm) norm[mine] = make_float2(m, outside ? NAN : 1.0f / s);
+    loss[mine] = ignored ? 0.f : (outside ? NAN : (m - label_logit[mine]) + logf(s));
   }
 }
 
@@ -784,6 +790,7 @@ int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, ProductAr
   // fp32 accumulator, both operands of the one 16-bit type, 256 x 256; MN-major operands at bits 15 and 16
   a.idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) |
             (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+  if (a.stage_bytes == 0) a.stage_bytes = 2 * kStageBytes;
   const long long slots = sm_count() / 2;
   const long long pairs = n_work < slots ? n_work : slots;
   cudaLaunchConfig_t cfg = {};
@@ -924,9 +931,13 @@ template <int MODE, bool FP16>
 int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats) {
   CUtensorMap map_a, map_b;
   const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
-  if (int rc = map_16(&map_a, h, x.hidden, n, x.ld_h, 128, FP16)) return rc;
+  // up to 128 rows: copies of those rows only (whole groups of eight, the swizzle's unit), none in the second CTA. Rows of a
+  // tile that nothing was copied to multiply whatever is there; their products are not used.
+  const int box = n <= 128 ? (int)up(n, 8) : 128;
+  if (int rc = map_16(&map_a, h, x.hidden, n, x.ld_h, box, FP16)) return rc;
   if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
   ProductArgs a = {};
+  a.stage_bytes = n <= 128 ? 2 * kOperandBytes + (uint32_t)box * 128 : 2 * kStageBytes;
   a.M = n;
   a.N = x.vocab;
   a.k_blocks = (int)((x.hidden + BK - 1) / BK);
