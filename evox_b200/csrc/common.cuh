@@ -42,6 +42,36 @@ void set_error(const char* fmt, ...);
     }                                                                                \
   } while (0)
 
+// ---------------------------------------------------------------------------
+// Launches that overlap the end of the kernel before them in the stream: the next grid's blocks may start
+// once every block of this one has started, and wait (overlapped_start, the first thing that they do) until the
+// grid before them has finished and its stores are visible. Every kernel launched by launch_overlapped calls it
+// in all threads, so that "finished" holds for everything earlier in the stream too.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void overlapped_start() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 int sm_count();  // cached multiprocessor count of the current device
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

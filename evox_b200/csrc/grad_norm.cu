@@ -153,6 +153,7 @@ __device__ __forceinline__ double block_sum_double(double x) {
 template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     grad_square_kernel(const __grid_constant__ Table<N> t, double* __restrict__ partial) {
+  overlapped_start();
   double sum = 0.0;
   const int chunks = t.begin[t.count];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -184,6 +185,7 @@ template <int N>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     grad_scale_kernel(const __grid_constant__ Table<N> t, const double* __restrict__ partial, int n_partial, float max_norm,
                       int write_norm, float* __restrict__ norm_out) {
+  overlapped_start();
   double sum = 0.0;
   for (int i = threadIdx.x; i < n_partial; i += kThreads) sum += partial[i];
   const float norm = (float)sqrt(block_sum_double(sum));
@@ -241,8 +243,7 @@ int launch_square(const Batch& b, const uint64_t* address, const int64_t* numel,
                   cudaStream_t stream) {
   Table<N> t;
   fill(t, b, address, numel, dtype, chunk_bytes);
-  grad_square_kernel<N><<<(unsigned)b.grid, kThreads, 0, stream>>>(t, partial);
-  EVOX_LAUNCH_CHECK();
+  EVOX_CUDA(launch_overlapped(grad_square_kernel<N>, dim3((unsigned)b.grid), kThreads, 0, 1, stream, t, partial));
   return EVOX_OK;
 }
 
@@ -251,8 +252,7 @@ int launch_scale(const Batch& b, const uint64_t* address, const int64_t* numel, 
                  int n_partial, float max_norm, int write_norm, float* norm, cudaStream_t stream) {
   Table<N> t;
   fill(t, b, address, numel, dtype, chunk_bytes);
-  grad_scale_kernel<N><<<(unsigned)b.grid, kThreads, 0, stream>>>(t, partial, n_partial, max_norm, write_norm, norm);
-  EVOX_LAUNCH_CHECK();
+  EVOX_CUDA(launch_overlapped(grad_scale_kernel<N>, dim3((unsigned)b.grid), kThreads, 0, 1, stream, t, partial, n_partial, max_norm, write_norm, norm));
   return EVOX_OK;
 }
 

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw);
   if ((smem_base & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned window: refuse to run otherwise
+    overlapped_start();
     if (threadIdx.x == 0) atomicCAS(a.error_flag, 0, 5);
     return;
   }
@@ -183,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // the peer's barriers exist before anything is sent to them
   fence_after_sync();
   const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+  overlapped_start();  // nothing of global memory was touched so far
 
   if (warp == 0) {
     // ------------------------------- TMA producer ------------------------------------------
@@ -527,6 +529,7 @@ __global__ void __launch_bounds__(1024)
     xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
                        const long long* __restrict__ labels, long long label_period, long long ignore_index, long long rows, long long vocab,
                        float2* __restrict__ norm, float* __restrict__ loss, const Weights weights) {
+  overlapped_start();
   if (weights.scalars && blockIdx.x == gridDim.x - 1) {  // one block more than the rows need
     row_weights(weights, ignore_index);
     return;
@@ -593,6 +596,7 @@ __global__ void __launch_bounds__(256)
                         float* __restrict__ bias_partial, const unsigned short* __restrict__ h, long long ld_h, long long hidden,
                         unsigned short* __restrict__ h_out, long long ld_h_out, int column_blocks, const float* __restrict__ loss, long long all_rows,
                         float* __restrict__ loss_out) {
+  overlapped_start();
   if ((int)blockIdx.y > column_blocks) {
     if (blockIdx.x == 0 && loss_out) sum_losses(loss, all_rows, scalars, loss_out);
     return;
@@ -720,6 +724,7 @@ struct BiasSum {
 };
 template <bool FP16>
 __global__ void __launch_bounds__(256) xent_join_kernel(const Join dh, const Join dw, const BiasSum db) {
+  overlapped_start();
   int block = blockIdx.x;
   if (block < db.blocks) {
     const long long v = (long long)block * 256 + threadIdx.x;
@@ -757,6 +762,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const Join dh, const Joi
 
 // Sum of the rows' losses times the reduction's factor: one block, 64-bit sums in a fixed order.
 __global__ void __launch_bounds__(256) xent_loss_sum_kernel(const float* __restrict__ loss, long long rows, const float* __restrict__ scalars, float* __restrict__ out) {
+  overlapped_start();
   sum_losses(loss, rows, scalars, out);
 }
 
@@ -793,20 +799,9 @@ int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, ProductAr
   if (a.stage_bytes == 0) a.stage_bytes = 2 * kStageBytes;
   const long long slots = sm_count() / 2;
   const long long pairs = n_work < slots ? n_work : slots;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, A_MN, B_MN, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
-  EVOX_CUDA(cudaLaunchKernelEx(&cfg, xent_product_kernel<MODE, A_MN, B_MN, FP16>, map_a, map_b, a));
+  EVOX_CUDA(launch_overlapped(xent_product_kernel<MODE, A_MN, B_MN, FP16>, dim3((unsigned)(2 * pairs)), kThreads, kSmemBytes, 2, stream, map_a,
+                              map_b, a));
   return EVOX_OK;
 }
 
@@ -920,9 +915,8 @@ struct Head {
 int finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
            long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const Weights& weights, cudaStream_t stream) {
   const int slices = (int)((vocab + kSlice - 1) / kSlice);
-  xent_finish_kernel<<<(unsigned)((rows + 31) / 32 + (weights.scalars ? 1 : 0)), 1024, 0, stream>>>(
-      stats, ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, weights);
-  EVOX_LAUNCH_CHECK();
+  EVOX_CUDA(launch_overlapped(xent_finish_kernel, dim3((unsigned)((rows + 31) / 32 + (weights.scalars ? 1 : 0))), 1024, 0, 1, stream, stats,
+                              ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, weights));
   return EVOX_OK;
 }
 
@@ -1012,11 +1006,10 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     const int column_blocks = (int)((x.vocab + 1023) / 1024), block_rows = rescale_rows(n, x.vocab);
     const int row_blocks = (int)((n + block_rows - 1) / block_rows);
     const bool sum_here = last && !per_row;
-    xent_rescale_kernel<FP16><<<dim3((unsigned)row_blocks, (unsigned)(column_blocks + (sum_here ? 2 : dw ? 1 : 0))), 256, 0, x.stream>>>(
-        b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss && per_row ? grad_loss + r0 : nullptr,
+    EVOX_CUDA(launch_overlapped(
+        xent_rescale_kernel<FP16>, dim3((unsigned)row_blocks, (unsigned)(column_blocks + (sum_here ? 2 : dw ? 1 : 0))), 256, 0, 1, x.stream, b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss && per_row ? grad_loss + r0 : nullptr,
         per_row, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, dw ? b.h_copy : nullptr, ld_copy,
-        column_blocks, row_loss, x.rows, sum_here ? loss : nullptr);
-    EVOX_LAUNCH_CHECK();
+        column_blocks, row_loss, x.rows, sum_here ? loss : nullptr));
     Join join_dh = {}, join_dw = {};
     CUtensorMap map_a, map_b;
     if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
@@ -1037,8 +1030,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     BiasSum bias = {};
     if (db) bias = BiasSum{b.bias_partial, db, b.scalars, x.vocab, row_blocks, !first, (int)((x.vocab + 255) / 256)};
     if (const int blocks = join_dh.blocks + join_dw.blocks + bias.blocks) {
-      xent_join_kernel<FP16><<<(unsigned)blocks, 256, 0, x.stream>>>(join_dh, join_dw, bias);
-      EVOX_LAUNCH_CHECK();
+      EVOX_CUDA(launch_overlapped(xent_join_kernel<FP16>, dim3((unsigned)blocks), 256, 0, 1, x.stream, join_dh, join_dw, bias));
     }
   }
   return EVOX_OK;
@@ -1077,8 +1069,7 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
   const Weights weights = {x.labels, rows, reduction, nullptr, 1.0f, per_row ? nullptr : b.scalars};
   if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, per_row ? loss : b.loss, weights, s)) return rc;
   if (!per_row) {
-    xent_loss_sum_kernel<<<1, 256, 0, s>>>(b.loss, rows, b.scalars, loss);
-    EVOX_LAUNCH_CHECK();
+    EVOX_CUDA(launch_overlapped(xent_loss_sum_kernel, dim3(1), 256, 0, 1, s, b.loss, rows, b.scalars, loss));
   }
   return EVOX_OK;
 }
