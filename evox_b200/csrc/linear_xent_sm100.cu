@@ -37,37 +37,37 @@ constexpr int kThreads = 64 + 256;
 constexpr int kChunkBlocks = 16;  // blocks of the reduction per accumulator of a logit
 constexpr uint32_t kOperandBytes = 128 * BK * 2;
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-constexpr uint32_t kOffBars = STAGES * kStageBytes;
-constexpr uint32_t kOffStage = kOffBars + 256;  // a warp's 32 x 32 values on their way to rows that start anywhere
-constexpr int kStagePitch = 34;
-constexpr uint32_t kSmemBytes = kOffStage + 8 * 32 * kStagePitch * 2;
+// half of a warp's 32 x 128 results on its way out: a swizzled tile of 32 rows x 128 bytes
+constexpr uint32_t kOffOut = STAGES * kStageBytes;
+constexpr uint32_t kOutBytes = 32 * 64 * 2;
+constexpr uint32_t kOffBars = kOffOut + 8 * kOutBytes;
+constexpr uint32_t kSmemBytes = kOffBars + 256;  // 229,632 B of the 232,448 B a CTA may use
 
-enum { kLoss = 0, kProb = 1, kOut = 2 };
+// What the epilogue leaves: kLoss the softmax statistics, kProb the exponentials too, kProbLow also what their rounding to
+// 16 bits left, kOut the product itself.
+enum { kLoss = 0, kProb = 1, kOut = 2, kProbLow = 3 };
 
 struct ProductArgs {
   long long M, N;
   int k_blocks;            // of BK
   int splits;              // the reduction is divided among this many work items per tile (kOut)
-  int chunks;              // accumulators that a tile's reduction is divided among (kLoss, kProb)
+  int chunks;              // accumulators that a tile's reduction is divided among (all but kOut)
   int tiles_m, tiles_n;
   uint32_t stage_bytes;    // what the copies of a stage bring to both CTAs
   int m_fast, group;       // tiles run through `group` of the one direction, then all of the other
   uint32_t idesc;
   int* error_flag;
-  // kLoss, kProb
+  // all but kOut
   const float* bias;       // [N] or null
   const long long* labels; // [M]
   float2* stats;           // [slices][ld_stats]: (maximum, sum of exponentials)
   long long ld_stats;
   float* label_logit;      // [M]
-  void* e;                 // [M][ld_e], kProb
-  void* e_low;             // what the rounding of e left, or null
-  long long ld_e;
   // kOut
   void* out16;             // [M][ld_out] (final), or null
   float* out32;            // [splits][M][ld32] partial sums, or the running sum over row chunks, or null
   long long ld_out, ld32;
-  int vec16;               // rows of out16 start on 32-byte boundaries
+  int tiled_out;           // out16 has a tensor map (rows on 16-byte boundaries)
   int add32;               // add what out32 holds before storing (or to out16)
   const float* scale;      // device scalar
 };
@@ -92,23 +92,55 @@ __device__ __forceinline__ float2 unpack2(uint32_t p) {
   if constexpr (FP16) return __half22float2(*reinterpret_cast<const __half2*>(&p));
   else return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
 }
-// Sixteen of a thread's values, from z[j] on, as 16 bits to a 32-byte aligned place.
-template <bool FP16>
-__device__ __forceinline__ void store_packed16(unsigned short* to, const float (&z)[32], int j, float scale) {
-  uint32_t p[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p[i] = pack2<FP16>(z[j + 2 * i] * scale, z[j + 2 * i + 1] * scale);
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
-               "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
-               : "memory");
-}
-template <bool FP16>
-__device__ __forceinline__ void store_packed(unsigned short* to, const float (&z)[32], float scale) {
-  store_packed16<FP16>(to, z, 0, scale);
-  store_packed16<FP16>(to + 16, z, 16, scale);
-}
 template <bool FP16>
 constexpr float kProbScale = FP16 ? 32768.0f : 1.0f;
+
+// 32 bytes to an aligned place.
+__device__ __forceinline__ void store_32_bytes(float* to, const float (&p)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(p[0]), "f"(p[1]), "f"(p[2]), "f"(p[3]),
+               "f"(p[4]), "f"(p[5]), "f"(p[6]), "f"(p[7])
+               : "memory");
+}
+
+// Place of 16-byte piece `piece` (0..7) of row `row` (0..31) in a warp's outgoing tile of 128-byte rows, with the 128-byte
+// swizzle of its tensor map; neighbouring rows' pieces fall into different banks.
+__device__ __forceinline__ uint32_t out_place(int row, int piece) { return (uint32_t)(row * 128 + ((piece ^ (row & 7)) << 4)); }
+// This thread's row (64 values, scaled) into the warp's outgoing tile. LOW: z becomes what the rounding left.
+template <bool FP16, bool LOW = false>
+__device__ __forceinline__ void put_row(uint8_t* out, int lane, float (&za)[32], float (&zb)[32], float scale) {
+#pragma unroll
+  for (int j = 0; j < 64; j += 8) {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float &a = j < 32 ? za[j + 2 * i] : zb[j - 32 + 2 * i], &b = j < 32 ? za[j + 2 * i + 1] : zb[j - 32 + 2 * i + 1];
+      p[i] = pack2<FP16>(a * scale, b * scale);
+      if constexpr (LOW) {
+        const float2 kept = unpack2<FP16>(p[i]);
+        a = fmaf(a, scale, -kept.x);
+        b = fmaf(b, scale, -kept.y);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + out_place(lane, j / 8)) = make_uint4(p[0], p[1], p[2], p[3]);
+  }
+}
+// The warp's tile to rows from `row` on and columns from `col` on of the map's matrix, which cuts off what lies outside.
+__device__ __forceinline__ void send_rows(const CUtensorMap* map, uint8_t* out, int lane, int col, int row) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((unsigned long long)map),
+                 "r"(smem_u32(out)), "r"(col), "r"(row)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// Until the copy that was sent has read the warp's tile.
+__device__ __forceinline__ void wait_sent(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+
 
 // Operand descriptor of an MN-major tile: 64 elements of the row direction are contiguous (128 bytes, swizzled), one
 // such line per reduction index; 8 lines make 1,024 bytes, the next 64 row elements start 64 lines further.
@@ -137,7 +169,8 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& a, long long work) {
 // D = A B^T over the reduction index; A_MN / B_MN: that operand is contiguous along its own rows instead.
 template <int MODE, bool A_MN, bool B_MN, bool FP16>
 __global__ void __launch_bounds__(kThreads, 1)
-    xent_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+    xent_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_low, const ProductArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw);
   if ((smem_base & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned window: refuse to run otherwise
@@ -299,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;          // TMEM lanes this warp may read
     const int half = (warp - 2) >> 2;      // which 128 of the tile's 256 columns this warp handles
     const uint32_t leader_tempty0 = map_to_cta(tempty_bar(0), 0u);
+    uint8_t* out = smem_raw + kOffOut + (warp - 2) * kOutBytes;
     long long it = 0;
     for (long long work = first; work < n_work; work += step) {
       const Tile t = tile_of(a, work);
@@ -345,53 +379,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (MODE == kOut) {
         const float scale = a.scale ? __ldg(a.scale) : 1.0f;
         float* o32 = a.out32 ? a.out32 + ((long long)t.split * a.M + row) * a.ld32 + col0 : nullptr;
-        unsigned short* o16 = a.out16 ? reinterpret_cast<unsigned short*>(a.out16) + row * a.ld_out + col0 : nullptr;
-        if (o32 && live) {  // rows of out32 hold a multiple of four columns
+        if (o32 && live) {  // rows of out32 hold a multiple of eight columns
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
+            for (int j = 0; j < 32; j += 8) {
               if (c * 32 + j < width) {
-                float4 r = make_float4(z[c][j] * scale, z[c][j + 1] * scale, z[c][j + 2] * scale, z[c][j + 3] * scale);
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = z[c][j + i] * scale;
                 if (a.add32) {
-                  const float4 b = *reinterpret_cast<const float4*>(o32 + c * 32 + j);
-                  r.x += b.x; r.y += b.y; r.z += b.z; r.w += b.w;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] += o32[c * 32 + j + i];
                 }
-                if (!o16) *reinterpret_cast<float4*>(o32 + c * 32 + j) = r;
-                z[c][j] = r.x; z[c][j + 1] = r.y; z[c][j + 2] = r.z; z[c][j + 3] = r.w;
+                if (!a.out16) store_32_bytes(o32 + c * 32 + j, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[c][j + i] = v[i];
               }
             }
         }
-        if (o16 && live) {
+        if (a.out16) {
+          const long long row0 = row - lane;
           const float s16 = o32 ? 1.0f : scale;
-          if (a.vec16) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c * 32 + 32 <= width) {
-                store_packed<FP16>(o16 + c * 32, z[c], s16);
-              } else {
+          for (int half64 = 0; half64 < 2; ++half64) {
+            if (half64 * 64 >= width || row0 >= a.M) break;
+            wait_sent(lane);
+            put_row<FP16>(out, lane, z[2 * half64], z[2 * half64 + 1], s16);
+            if (a.tiled_out) {
+              send_rows(&map_out, out, lane, (int)col0 + half64 * 64, (int)row0);
+            } else {  // rows that start anywhere: row by row, lanes along it
+              __syncwarp();
+              unsigned short* to = reinterpret_cast<unsigned short*>(a.out16) + row0 * a.ld_out + col0 + half64 * 64;
+              const int rows_here = (int)min(32ll, a.M - row0);
+              for (int i = 0; i < rows_here; ++i)
 #pragma unroll
-                for (int j = 0; j < 32; j += 16)  // rows hold a multiple of 16 columns
-                  if (c * 32 + j < width) store_packed16<FP16>(o16 + c * 32 + j, z[c], j, s16);
-              }
+                for (int c = lane; c < 64; c += 32)
+                  if (half64 * 64 + c < width)
+                    to[i * a.ld_out + c] = *reinterpret_cast<const unsigned short*>(out + out_place(i, c >> 3) + (c & 7) * 2);
             }
-          }
-        }
-        if (o16 && !a.vec16) {
-          // rows that start anywhere: 32 x 32 values pass through shared memory and leave row by row, lanes along it
-          const float s16 = o32 ? 1.0f : scale;
-          unsigned short* stage = reinterpret_cast<unsigned short*>(smem_raw + kOffStage) + (warp - 2) * (32 * kStagePitch);
-          unsigned short* tile16 = reinterpret_cast<unsigned short*>(a.out16) + (row - lane) * a.ld_out + col0;
-          const int rows_here = (int)max(0ll, min(32ll, a.M - (row - lane)));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              *reinterpret_cast<uint32_t*>(stage + lane * kStagePitch + j) = pack2<FP16>(z[c][j] * s16, z[c][j + 1] * s16);
-            __syncwarp();
-            if (c * 32 + lane < width)
-              for (int i = 0; i < rows_here; ++i) tile16[i * a.ld_out + c * 32 + lane] = stage[i * kStagePitch + lane];
           }
         }
       } else {
@@ -439,25 +465,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (live && width > 0)
           a.stats[(long long)(t.n * 2 + half) * a.ld_stats + row] = make_float2(m, (part[0] + part[1]) + (part[2] + part[3]));
-        if constexpr (MODE == kProb) {
-          unsigned short* e = reinterpret_cast<unsigned short*>(a.e) + row * a.ld_e + col0;
+        if constexpr (MODE != kLoss) {
+          const long long row0 = row - lane;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (live && col0 + c * 32 < a.ld_e) {  // rows of e hold a multiple of 64 columns
-              store_packed<FP16>(e + c * 32, z[c], kProbScale<FP16>);
-              if (a.e_low) {
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                  const float2 kept = unpack2<FP16>(pack2<FP16>(z[c][j] * kProbScale<FP16>, z[c][j + 1] * kProbScale<FP16>));
-                  z[c][j] = fmaf(z[c][j], kProbScale<FP16>, -kept.x);
-                  z[c][j + 1] = fmaf(z[c][j + 1], kProbScale<FP16>, -kept.y);
-                }
-                store_packed<FP16>(reinterpret_cast<unsigned short*>(a.e_low) + row * a.ld_e + col0 + c * 32, z[c], 1.0f);
-              }
+          for (int half64 = 0; half64 < 2; ++half64) {
+            if (half64 * 64 >= width || row0 >= a.M) break;
+            wait_sent(lane);
+            put_row<FP16, MODE == kProbLow>(out, lane, z[2 * half64], z[2 * half64 + 1], kProbScale<FP16>);
+            send_rows(&map_out, out, lane, (int)col0 + half64 * 64, (int)row0);
+            if constexpr (MODE == kProbLow) {
+              wait_sent(lane);
+              put_row<FP16>(out, lane, z[2 * half64], z[2 * half64 + 1], 1.0f);
+              send_rows(&map_low, out, lane, (int)col0 + half64 * 64, (int)row0);
             }
+          }
         }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   fence_before_sync();
   __syncthreads();
@@ -630,7 +655,9 @@ __global__ void __launch_bounds__(256)
   __shared__ float weight[32];
   __shared__ int target[32];
   __shared__ float sums[128][8];
-  const long long col_base = (long long)blockIdx.y * 1024;
+  // backwards: the columns that the product wrote last are still in the L2 cache, and those written here last are the first
+  // that the next product reads
+  const long long col_base = (long long)(column_blocks - 1 - (int)blockIdx.y) * 1024;
   {  // one (row, slice) per thread
     const int r = tid & 31, s = tid >> 5;
     const long long slice = col_base / kSlice + s;
@@ -787,7 +814,8 @@ int map_16(CUtensorMap* map, const void* base, long long inner, long long outer,
 }
 
 template <int MODE, bool A_MN, bool B_MN, bool FP16>
-int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, ProductArgs& a, cudaStream_t stream) {
+int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_out, const CUtensorMap& map_low, ProductArgs& a,
+                   cudaStream_t stream) {
   a.tiles_m = (int)((a.M + TM - 1) / TM);
   a.tiles_n = (int)((a.N + TN - 1) / TN);
   const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
@@ -801,7 +829,7 @@ int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, ProductAr
   const long long pairs = n_work < slots ? n_work : slots;
   EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, A_MN, B_MN, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
   EVOX_CUDA(launch_overlapped(xent_product_kernel<MODE, A_MN, B_MN, FP16>, dim3((unsigned)(2 * pairs)), kThreads, kSmemBytes, 2, stream, map_a,
-                              map_b, a));
+                              map_b, map_out, map_low, a));
   return EVOX_OK;
 }
 
@@ -874,12 +902,12 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
     size_t part_dh = 0;
     for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
       const int splits = reduction_splits(r, hidden, vocab);
-      if (splits > 1 && part_dh < (size_t)splits * r * up(hidden, 4)) part_dh = (size_t)splits * r * up(hidden, 4);
+      if (splits > 1 && part_dh < (size_t)splits * r * up(hidden, 8)) part_dh = (size_t)splits * r * up(hidden, 8);
     }
     const int splits_dw = chunk < rows ? 1 : reduction_splits(vocab, hidden, rows);
     b.partial_dh = part_dh ? c.take<float>(part_dh) : nullptr;
-    b.partial_dw = splits_dw > 1 ? c.take<float>((size_t)splits_dw * vocab * up(hidden, 4)) : nullptr;
-    b.dw_sum = chunk < rows ? c.take<float>((size_t)vocab * up(hidden, 4)) : nullptr;
+    b.partial_dw = splits_dw > 1 ? c.take<float>((size_t)splits_dw * vocab * up(hidden, 8)) : nullptr;
+    b.dw_sum = chunk < rows ? c.take<float>((size_t)vocab * up(hidden, 8)) : nullptr;
   }
   return c.used;
 }
@@ -920,7 +948,7 @@ int finish(const float2* stats, long long ld_stats, const float* label_logit, co
   return EVOX_OK;
 }
 
-// Logits of `n` rows from `r0` on: (maximum, sum) per slice, the labels' logits, and with MODE == kProb the exponentials.
+// Logits of `n` rows from `r0` on: (maximum, sum) per slice, the labels' logits, and the exponentials, as MODE says.
 template <int MODE, bool FP16>
 int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats) {
   CUtensorMap map_a, map_b;
@@ -947,10 +975,14 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
   a.stats = b.stats;
   a.ld_stats = ld_stats;
   a.label_logit = b.label_logit;
-  a.e = MODE == kProb ? b.e : nullptr;
-  a.e_low = MODE == kProb ? b.e_low : nullptr;
-  a.ld_e = up(x.vocab, 64);
-  return launch_product<MODE, false, false, FP16>(map_a, map_b, a, x.stream);
+  CUtensorMap map_e = map_a, map_low = map_a;  // not used without exponentials
+  if (MODE != kLoss) {
+    const long long ld_e = up(x.vocab, 64);
+    if (int rc = map_16(&map_e, b.e, x.vocab, n, ld_e, 32, FP16)) return rc;
+    if (MODE == kProbLow)
+      if (int rc = map_16(&map_low, b.e_low, x.vocab, n, ld_e, 32, FP16)) return rc;
+  }
+  return launch_product<MODE, false, false, FP16>(map_a, map_b, map_e, map_low, a, x.stream);
 }
 
 // out (M x N, 16 bits, dense) = scale * A B^T with the reduction divided where that fills the machine better.
@@ -969,8 +1001,7 @@ int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long lo
   a.error_flag = error_flag;
   a.scale = scale;
   a.ld_out = N;
-  a.ld32 = up(N, 4);
-  a.vec16 = N % 16 == 0 && ((uintptr_t)out & 31u) == 0;
+  a.ld32 = up(N, 8);
   if (sum) {
     a.out32 = sum;
     a.add32 = !first;
@@ -980,7 +1011,11 @@ int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long lo
   } else {
     a.out16 = out;
   }
-  if (int rc = launch_product<kOut, A_MN, true, FP16>(map_a, map_b, a, stream)) return rc;
+  CUtensorMap map_out = map_a;
+  a.tiled_out = a.out16 && N % 8 == 0 && aligned16(out);
+  if (a.tiled_out)
+    if (int rc = map_16(&map_out, out, N, M, N, 32, FP16)) return rc;
+  if (int rc = launch_product<kOut, A_MN, true, FP16>(map_a, map_b, map_out, map_out, a, stream)) return rc;
   if (a.splits > 1) {
     const long long blocks = (M * ((N + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
     *join = Join{partial, reinterpret_cast<unsigned short*>(out), M, N, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
@@ -998,7 +1033,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
   for (long long r0 = 0; r0 < x.rows; r0 += chunk) {
     const long long n = x.rows - r0 < chunk ? x.rows - r0 : chunk;
     const bool first = r0 == 0, last = r0 + n == x.rows;
-    if (int rc = logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
+    if (int rc = b.e_low ? logits_pass<kProbLow, FP16>(x, b, r0, n, chunk) : logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
     const Weights weights = {x.labels, x.rows, reduction, grad_loss, kProbScale<FP16>, first ? b.scalars : nullptr};
     if (int rc = finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, row_loss + r0, weights, x.stream))
       return rc;
