@@ -224,39 +224,41 @@ def lora_layer_cross_entropy(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tens
     The epilogue reduces the logits to softmax statistics, so (pop, batch, vocab) never exists. A token labelled `ignore_index`
     has loss 0, another label outside the vocabulary gives NaN."""
     rank = 8
+    err = _cabi.EvoxKernelError
     if h.ndim != 3 or w.ndim != 2 or h.shape[2] != w.shape[1]:
-        raise _cabi.EvoxKernelError(f"shape mismatch: h {tuple(h.shape)}, w {tuple(w.shape)}")
+        raise err(f"shape mismatch: h {tuple(h.shape)}, w {tuple(w.shape)}")
     pop, batch, k = h.shape
     vocab = w.shape[0]
-    dev = h.device
     if h.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
-        raise _cabi.EvoxKernelError("lora_layer_cross_entropy needs bf16 activations and weights")
+        raise err("lora_layer_cross_entropy needs bf16 activations and weights")
     seeds = _seeds(seeds)
     if seeds.shape[0] != pop or labels.dtype != torch.int64 or labels.shape != (batch,):
-        raise _cabi.EvoxKernelError(f"needs {pop} seeds and int64 labels of shape ({batch},), got {seeds.shape[0]} and {labels.dtype} {tuple(labels.shape)}")
+        raise err(f"needs {pop} seeds and int64 labels of shape ({batch},), got {seeds.shape[0]} and {labels.dtype} {tuple(labels.shape)}")
     if bias is not None and bias.shape != (vocab,):
-        raise _cabi.EvoxKernelError(f"bias must have shape ({vocab},), got {tuple(bias.shape)}")
+        raise err(f"bias must have shape ({vocab},), got {tuple(bias.shape)}")
     if t is not None and (t.shape != (pop, batch, rank) or t.dtype != torch.float32):
-        raise _cabi.EvoxKernelError(f"t must be fp32 of shape ({pop}, {batch}, {rank}), got {t.dtype} {tuple(t.shape)}")
-    if not _cabi.lib.evox_lora_cross_entropy_supported(pop, batch, k, vocab, rank):
-        raise _cabi.EvoxKernelError(f"layer shape (pop {pop}, batch {batch}, k {k}, vocab {vocab}) is not supported by the tensor-core path")
+        raise err(f"t must be fp32 of shape ({pop}, {batch}, {rank}), got {t.dtype} {tuple(t.shape)}")
+    lib = _cabi.lib
+    if not lib.evox_lora_cross_entropy_supported(pop, batch, k, vocab, rank):
+        raise err(f"layer shape (pop {pop}, batch {batch}, k {k}, vocab {vocab}) is not supported by the tensor-core path")
+    dev = h.device
+    s = _cabi.stream_ptr(dev) if h.is_cuda else None  # ptr() refuses what is not on the current CUDA device
     h, w, labels = h.contiguous(), w.contiguous(), labels.contiguous()
-    lib, s = _cabi.lib, _cabi.stream_ptr(dev)
-    if t is not None:
-        t = t.contiguous()
-    else:
-        t = torch.empty(pop, batch, rank, dtype=torch.float32, device=dev)
-        _cabi.check(lib.evox_lora_down_bf16(_cabi.ptr(h), _cabi.ptr(seeds), counter, pop, batch, k, rank, _cabi.ptr(t), s))
+    h_ptr, w_ptr, seeds_ptr = _cabi.ptr(h), _cabi.ptr(w), _cabi.ptr(seeds)
     bias_f = None if bias is None else bias.to(device=dev, dtype=torch.float32).contiguous()
+    if t is None:
+        t = torch.empty(pop, batch, rank, dtype=torch.float32, device=dev)
+        _cabi.check(lib.evox_lora_down_bf16(h_ptr, seeds_ptr, counter, pop, batch, k, rank, t.data_ptr(), s))
+    else:
+        t = t.contiguous()
     loss = torch.empty(pop, batch, dtype=torch.float32, device=dev)
     nbytes = lib.evox_lora_cross_entropy_workspace_bytes(pop, batch, vocab)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    err = status_word(dev)
     _cabi.check(
         lib.evox_lora_cross_entropy_bf16(
-            _cabi.ptr(h), _cabi.ptr(w), _cabi.ptr(bias_f), _cabi.ptr(t), _cabi.ptr(seeds), counter + _ceil4(rank * k),
-            int(bias is not None and bias_counter is not None), bias_counter or 0, float(sigma), pop, batch, k, vocab, rank,
-            _cabi.ptr(labels), ignore_index, _cabi.ptr(loss), _cabi.ptr(ws), nbytes, _cabi.ptr(err), s,
+            h_ptr, w_ptr, _cabi.ptr(bias_f), _cabi.ptr(t), seeds_ptr, counter + _ceil4(rank * k), int(bias is not None and bias_counter is not None),
+            bias_counter or 0, float(sigma), pop, batch, k, vocab, rank, _cabi.ptr(labels), ignore_index, loss.data_ptr(), ws.data_ptr(),
+            nbytes, status_word(dev).data_ptr(), s,
         )
     )
     return loss
