@@ -495,6 +495,316 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows (up to 64). The product is bound by reading the weight once, so the operands change sides: 256 rows of the long
+// operand (the weight's, or its columns for dh) fill the tensor core's rows and the tokens are its 32 or 64 columns. A
+// block of the reduction then takes an eighth of the tensor cycles of a tile with 256 columns, and the ring holds
+// nearly nothing but the weight (ten stages). Accumulator lanes are weight rows, so the softmax statistics of a token
+// run across lanes and the four warps that share a slice of 128.
+// ---------------------------------------------------------------------------------------------
+constexpr int kFewRows = 64;
+constexpr int kFewChunkBlocks = 4;  // accumulators are small and the tensor core has time: join them more often
+constexpr int kFewStages = 10;
+constexpr uint32_t kFewStageBytes = kOperandBytes + 32 * 128;  // 128 lines of the long operand, up to 32 tokens' of the short one
+constexpr uint32_t kFewOffBars = kFewStages * kFewStageBytes;
+constexpr uint32_t kFewOffShared = kFewOffBars + 256;          // float [2: maxima, sums][2 halves][4 warps][32 tokens]
+constexpr uint32_t kFewSmemBytes = kFewOffShared + 2 * 2 * 4 * 32 * 4;
+
+struct FewArgs {
+  long long M;             // rows of the long operand: words, or hidden features
+  int rows;                // tokens
+  int k_blocks, splits, chunks, tiles;
+  uint32_t idesc;
+  int* error_flag;
+  // all but kOut
+  const float* bias;
+  const long long* labels;
+  float2* stats;
+  long long ld_stats;
+  float* label_logit;
+  unsigned short* e;       // [rows][ld_e]
+  unsigned short* e_low;
+  long long ld_e;
+  // kOut
+  unsigned short* out16;   // [rows][M], or null
+  float* out32;            // [splits][rows][ld32], or null
+  long long ld32;
+  const float* scale;
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Across the warp: lane l gets the maximum or the sum over all lanes of v[l % T]. Halves of the values change hands in every step,
+// so T values cost T - 1 exchanges (and T more for T = 16, whose first step keeps them all).
+template <int T, bool MAX>
+__device__ __forceinline__ float reduce_lanes(const float (&x)[T], int lane) {
+  float v[T];
+#pragma unroll
+  for (int j = 0; j < T; ++j) v[j] = x[j];
+  auto join = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+#pragma unroll
+  for (int step = 16; step >= T; step >>= 1)
+#pragma unroll
+    for (int j = 0; j < T; ++j) v[j] = join(v[j], __shfl_xor_sync(0xffffffffu, v[j], step));
+#pragma unroll
+  for (int step = T / 2; step > 0; step >>= 1) {
+    const bool high = lane & step;
+#pragma unroll
+    for (int j = 0; j < step; ++j) {
+      const float give = high ? v[j] : v[j + step], keep = high ? v[j + step] : v[j];
+      v[j] = join(keep, __shfl_xor_sync(0xffffffffu, give, step));
+    }
+  }
+  return v[0];
+}
+
+template <int MODE, bool A_MN, bool FP16, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+    xent_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const FewArgs a) {
+  constexpr int T = NT / 2;  // tokens of one of the two warp groups
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = smem_u32(smem_raw);
+  if ((smem_base & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned window: refuse to run otherwise
+    overlapped_start();
+    if (threadIdx.x == 0) atomicCAS(a.error_flag, 0, 5);
+    return;
+  }
+  const uint32_t bars = smem_base + kFewOffBars;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (kFewStages + s); };
+  auto tfull_bar = [&](int b) { return bars + 8u * (2 * kFewStages + b); };
+  auto tempty_bar = [&](int b) { return bars + 8u * (2 * kFewStages + 2 + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + kFewOffBars + 8 * (2 * kFewStages + 4));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_rank();
+  const int n_work = a.tiles * a.splits, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int chunks = MODE == kOut ? 1 : a.chunks;
+  auto split_begin = [&](int split) { return (int)((long long)split * a.k_blocks / a.splits); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers exist before anything is sent to them
+  fence_after_sync();
+  const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
+  overlapped_start();  // nothing of global memory was touched so far
+
+  if (warp == 0) {
+    if (lane == 0) {  // TMA producer
+      int s = 0;
+      uint32_t ph = 0, issued = 0;
+      bool ok = true;
+      const uint32_t leader_full0 = map_to_cta(full_bar(0), 0u);
+      for (int work = first; work < n_work && ok; work += step) {
+        const int split = work / a.tiles, m0 = (work - split * a.tiles) * 256 + (int)cta_rank * 128;
+        for (int kb = split_begin(split); kb < split_begin(split + 1); ++kb) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) {
+            ok = false;
+            break;
+          }
+          if (cta_rank == 0) mbar_expect_tx(full_bar(s), 2 * kOperandBytes + NT * 128);
+          const uint32_t fb = leader_full0 + 8u * s, sa = smem_base + s * kFewStageBytes, sb = sa + kOperandBytes;
+          const int k0 = kb * BK;
+          if constexpr (A_MN) {
+            tma_load_2d_pair(sa, &map_a, fb, m0, k0);
+            tma_load_2d_pair(sa + kOperandBytes / 2, &map_a, fb, m0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sa, &map_a, fb, k0, m0);
+          }
+          tma_load_2d_pair(sb, &map_b, fb, k0, (int)cta_rank * T);
+          issued |= 1u << s;
+          if (++s == kFewStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // the leader's releases of this CTA's stages arrive asynchronously: see the last one of every stage land
+      for (int q = 0; q < kFewStages && ok; ++q) {
+        if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) ok = false;
+        if (++s == kFewStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if (!ok) {  // as in xent_product_kernel: nothing may be under way when shared memory is released
+        for (int q = 0; q < kFewStages && cta_rank == 0; ++q) {
+          if (!(issued & (1u << q))) continue;
+          const uint32_t last = (q < s) ? ph : (ph ^ 1u);
+          const unsigned long long t0 = global_timer_ns();
+          while (!mbar_try(full_bar(q), last) && !mbar_try(full_bar(q), last ^ 1u)) {
+            if (global_timer_ns() - t0 > kWaitLimitNs) break;
+          }
+        }
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cta_rank == 0) {  // MMA issuer
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int work = first; work < n_work && ok; work += step) {
+        const int split = work / a.tiles, begin = split_begin(split), count = split_begin(split + 1) - begin;
+        for (int chunk = 0; chunk < chunks && ok; ++chunk, ++it) {
+          const int buf = it & 1;
+          if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          const uint32_t d_tmem = tmem_base + (uint32_t)(buf * NT);
+          const int kb0 = chunk * count / chunks, kb1 = (chunk + 1) * count / chunks;
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
+              ok = false;
+              break;
+            }
+            fence_after_sync();
+            const uint32_t sa = smem_base + s * kFewStageBytes, sb = sa + kOperandBytes;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              umma_f16_pair(d_tmem, A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32), umma_desc(sb + k * 32), a.idesc,
+                            (kb > kb0 || k > 0) ? 1u : 0u);
+            umma_commit_pair(empty_bar(s));
+            if (++s == kFewStages) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+          if (ok) umma_commit_pair(tfull_bar(buf));
+        }
+      }
+    }
+  } else {
+    // epilogue: lanes are rows of the long operand, warps 2-5 and 6-9 take half of the tokens each
+    const int quarter = warp & 3, half = (warp - 2) >> 2, token0 = half * T;
+    const uint32_t leader_tempty0 = map_to_cta(tempty_bar(0), 0u);
+    float* maxima = reinterpret_cast<float*>(smem_raw + kFewOffShared) + half * (4 * 32);
+    float* sums = maxima + 2 * 4 * 32;
+    const int live_tokens = max(0, min(T, a.rows - token0));
+    long long label = -1;
+    if constexpr (MODE != kOut)
+      if (lane < live_tokens) label = __ldg(a.labels + token0 + lane);  // of the lane's token
+    int it = 0;
+    bool ok = true;  // after a wait that gave up a warp does no work, but meets the others at their barriers
+    for (int work = first; work < n_work; work += step) {
+      const int split = work / a.tiles;
+      const long long base = (long long)(work - split * a.tiles) * 256 + cta_rank * 128 + quarter * 32, row = base + lane;
+      const bool live = row < a.M;
+      float bias = 0.f;
+      if constexpr (MODE != kOut)
+        if (a.bias && live) bias = __ldg(a.bias + row);
+      float z[T];
+      for (int chunk = 0; chunk < chunks && ok; ++chunk, ++it) {
+        const int buf = it & 1;
+        ok = mbar_wait(tfull_bar(buf), (uint32_t)((it >> 1) & 1), a.error_flag, 4);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after_sync();
+        uint32_t v[T];
+        const uint32_t taddr = tmem_base + (uint32_t)(buf * NT + token0) + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+        for (int j = 0; j < T; j += 16) tmem_ld16(taddr + j, v + j);
+        tmem_ld_wait();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8u * buf);
+#pragma unroll
+        for (int j = 0; j < T; ++j) z[j] = chunk == 0 ? __uint_as_float(v[j]) : z[j] + __uint_as_float(v[j]);
+      }
+      if constexpr (MODE == kOut) {
+        if (!ok) break;
+        const float scale = a.scale ? __ldg(a.scale) : 1.0f;
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < T; ++j) {
+            if (j >= live_tokens) break;
+            if (a.out32) a.out32[((long long)split * a.rows + token0 + j) * a.ld32 + row] = z[j] * scale;
+            else a.out16[(long long)(token0 + j) * a.M + row] = pack1<FP16>(z[j] * scale);
+          }
+        }
+      } else {
+        if (!ok) {
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < T; ++j) z[j] = live ? z[j] + bias : -INFINITY;
+        const long long at = label - base;  // lane of this warp that holds the lane's token's label
+        if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+#pragma unroll
+          for (int j = 0; j < T; ++j) {
+            const long long where = __shfl_sync(0xffffffffu, at, j);
+            if (j < live_tokens && where == lane && live) a.label_logit[token0 + j] = z[j];
+          }
+        }
+        const float warp_max = reduce_lanes<T, true>(z, lane);
+        if (lane < T) maxima[quarter * 32 + lane] = warp_max;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        float m = -INFINITY;  // of the lane's token (lane % T) over the slice
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, maxima[q * 32 + (lane & (T - 1))]);
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+          const float top = __shfl_sync(0xffffffffu, m, j);
+          z[j] = exp2_approx((z[j] - (top == -INFINITY ? 0.f : top)) * kLog2e);
+        }
+        const float warp_sum32 = reduce_lanes<T, false>(z, lane);
+        if (lane < T) sums[quarter * 32 + lane] = warp_sum32;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        if (quarter == 0 && lane < live_tokens && base < a.M) {
+          const float s = (sums[lane] + sums[32 + lane]) + (sums[64 + lane] + sums[96 + lane]);
+          a.stats[(base / kSlice) * a.ld_stats + token0 + lane] = make_float2(m, s);
+        }
+        if constexpr (MODE != kLoss) {
+          if (live) {
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+              if (j >= live_tokens) break;
+              const unsigned short kept = pack1<FP16>(z[j] * kProbScale<FP16>);
+              const long long to = (long long)(token0 + j) * a.ld_e + row;
+              a.e[to] = kept;
+              if constexpr (MODE == kProbLow) a.e_low[to] = pack1<FP16>(fmaf(z[j], kProbScale<FP16>, -unpack2<FP16>(kept).x));
+            }
+          }
+        }
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the pair leaves together
+  if (warp == 1) {
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 128;" ::"r"(tmem_base) : "memory");
+  }
+}
+
 // What the rows count for, by one block of 1,024 threads (a fixed order, and the counts are whole numbers). `scalars`: [0]
 // scale of the gradient (the rows' weights are stored as fractions of the largest one, so that any upstream gradient
 // fits the 16-bit type), [1] the weights' inverse scale, [2] factor of the summed loss.
@@ -855,6 +1165,39 @@ int rescale_rows(long long rows, long long vocab) {
   return ((rows + 31) / 32) * ((vocab + 1023) / 1024) >= 4ll * sm_count() ? 32 : 8;
 }
 
+// Work items per tile of a product with few tokens: one item per CTA pair (four were slower: 183 against 174 us for a gradient
+// at 8 x 4,096 x 32,000), at least eight blocks of the reduction each.
+int few_splits(long long M, long long K) {
+  const long long tiles = (M + 255) / 256, pairs = sm_count() / 2, kb = (K + BK - 1) / BK;
+  long long s = pairs / tiles;
+  if (s > kb / 8) s = kb / 8;
+  return (int)(s < 1 ? 1 : s);
+}
+
+// Splits of dh for `rows` rows.
+int dh_splits(long long rows, long long hidden, long long vocab) {
+  return rows <= kFewRows ? few_splits(hidden, vocab) : reduction_splits(rows, hidden, vocab);
+}
+
+template <int MODE, bool A_MN, bool FP16, int NT>
+int launch_few_nt(const CUtensorMap& map_a, const CUtensorMap& map_b, FewArgs& a, cudaStream_t stream) {
+  a.tiles = (int)((a.M + 255) / 256);
+  a.idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) | (A_MN ? 1u << 15 : 0u);
+  const long long n_work = (long long)a.tiles * a.splits, slots = sm_count() / 2, pairs = n_work < slots ? n_work : slots;
+  EVOX_CUDA(cudaFuncSetAttribute(xent_few_kernel<MODE, A_MN, FP16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmemBytes));
+  EVOX_CUDA(launch_overlapped(xent_few_kernel<MODE, A_MN, FP16, NT>, dim3((unsigned)(2 * pairs)), kThreads, kFewSmemBytes, 2, stream, map_a, map_b, a));
+  return EVOX_OK;
+}
+
+// The long operand through `map_a`, `a.rows` tokens (K-major lines of `line` elements, `ld` apart).
+template <int MODE, bool A_MN, bool FP16>
+int launch_few(const CUtensorMap& map_a, const void* tokens, long long line, long long ld, FewArgs& a, cudaStream_t stream) {
+  CUtensorMap map_b;
+  const bool small = a.rows <= 32;
+  if (int rc = map_16(&map_b, tokens, line, a.rows, ld, small ? 16 : 32, FP16)) return rc;
+  return small ? launch_few_nt<MODE, A_MN, FP16, 32>(map_a, map_b, a, stream) : launch_few_nt<MODE, A_MN, FP16, 64>(map_a, map_b, a, stream);
+}
+
 struct Carve {  // 256-byte aligned pieces of the workspace
   uint8_t* base;
   size_t used;
@@ -901,7 +1244,7 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
     b.bias_partial = with_bias ? c.take<float>(sums * vocab) : nullptr;
     size_t part_dh = 0;
     for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
-      const int splits = reduction_splits(r, hidden, vocab);
+      const int splits = dh_splits(r, hidden, vocab);
       if (splits > 1 && part_dh < (size_t)splits * r * up(hidden, 8)) part_dh = (size_t)splits * r * up(hidden, 8);
     }
     const int splits_dw = chunk < rows ? 1 : reduction_splits(vocab, hidden, rows);
@@ -953,6 +1296,25 @@ template <int MODE, bool FP16>
 int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats) {
   CUtensorMap map_a, map_b;
   const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
+  if (n <= kFewRows) {
+    if (int rc = map_16(&map_a, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
+    FewArgs a = {};
+    a.M = x.vocab;
+    a.rows = (int)n;
+    a.k_blocks = (int)((x.hidden + BK - 1) / BK);
+    a.splits = 1;
+    a.chunks = (a.k_blocks + kFewChunkBlocks - 1) / kFewChunkBlocks;
+    a.error_flag = x.error_flag;
+    a.bias = x.bias;
+    a.labels = x.labels + r0;
+    a.stats = b.stats;
+    a.ld_stats = ld_stats;
+    a.label_logit = b.label_logit;
+    a.e = b.e;
+    a.e_low = b.e_low;
+    a.ld_e = up(x.vocab, 64);
+    return launch_few<MODE, false, FP16>(map_a, h, x.hidden, x.ld_h, a, x.stream);
+  }
   // up to 128 rows: copies of those rows only (whole groups of eight, the swizzle's unit), none in the second CTA. Rows of a
   // tile that nothing was copied to multiply whatever is there; their products are not used.
   const int box = n <= 128 ? (int)up(n, 8) : 128;
@@ -1047,7 +1409,25 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
         column_blocks, row_loss, x.rows, sum_here ? loss : nullptr));
     Join join_dh = {}, join_dw = {};
     CUtensorMap map_a, map_b;
-    if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
+    if (dh && n <= kFewRows) {
+      if (int rc = map_16(&map_a, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
+      FewArgs a = {};
+      a.M = x.hidden;
+      a.rows = (int)n;
+      a.k_blocks = (int)((x.vocab + BK - 1) / BK);
+      a.splits = few_splits(x.hidden, x.vocab);
+      a.error_flag = x.error_flag;
+      a.scale = b.scalars;
+      a.ld32 = up(x.hidden, 8);
+      unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;
+      if (a.splits > 1) a.out32 = b.partial_dh;
+      else a.out16 = out;
+      if (int rc = launch_few<kOut, true, FP16>(map_a, b.e, x.vocab, ld_e, a, x.stream)) return rc;
+      if (a.splits > 1) {
+        const long long blocks = (n * ((x.hidden + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
+        join_dh = Join{b.partial_dh, out, n, x.hidden, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
+      }
+    } else if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
       if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 128, FP16)) return rc;
       if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
       unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;

@@ -79,7 +79,8 @@ def near(got, want, tol, what):
 
 
 SIZES = [(1, 8, 1), (1, 64, 5), (2, 1, 3), (3, 100, 257), (64, 256, 1000), (129, 512, 1009), (255, 72, 128), (256, 64, 256), (257, 1000, 1023),
-         (300, 1001, 777), (1024, 256, 4099), (40, 4096, 300), (2000, 136, 70)]
+         (300, 1001, 777), (1024, 256, 4099), (40, 4096, 300), (2000, 136, 70), (65, 64, 300), (128, 200, 1000), (32, 96, 129), (33, 1001, 640),
+         (9, 2200, 2500)]
 
 
 @gpu
