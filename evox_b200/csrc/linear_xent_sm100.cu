@@ -922,8 +922,8 @@ __device__ void sum_losses(const float* __restrict__ loss, long long rows, const
 // rounding left. The blocks of one more grid row copy the hidden states for the weight gradient, with zeros where the
 // label is ignored: 0 x inf in a padded row must not reach dw. The first block of another one sums the losses of
 // all rows once they are there.
-template <bool FP16>
-__global__ void __launch_bounds__(256)
+template <bool FP16, bool BIAS>
+__global__ void __launch_bounds__(256, BIAS ? 3 : 5)
     xent_rescale_kernel(unsigned short* __restrict__ e, const unsigned short* __restrict__ e_low, long long ld_e,
                         const float2* __restrict__ stats, long long ld_stats, int slices, const float2* __restrict__ norm,
                         const long long* __restrict__ labels, long long ignore_index, const float* __restrict__ grad_loss, int per_row,
@@ -968,6 +968,17 @@ __global__ void __launch_bounds__(256)
   // backwards: the columns that the product wrote last are still in the L2 cache, and those written here last are the first
   // that the next product reads
   const long long col_base = (long long)(column_blocks - 1 - (int)blockIdx.y) * 1024;
+  const int group = tid & 127, part = tid >> 7;  // eight columns; even or odd rows
+  const long long col = col_base + group * 8;
+  unsigned short* column = e + row0 * ld_e + col;
+  // four rows at once; the first four are on their way while the factors are looked up
+  uint4 p[4];
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r0 + 2 * i < n_rows) p[i] = *reinterpret_cast<const uint4*>(column + (r0 + 2 * i) * ld_e);
+  };
+  if (col < ld_e) fetch(part);
   {  // one (row, slice) per thread
     const int r = tid & 31, s = tid >> 5;
     const long long slice = col_base / kSlice + s;
@@ -992,18 +1003,15 @@ __global__ void __launch_bounds__(256)
     }
   }
   __syncthreads();
-  const int group = tid & 127, part = tid >> 7;  // eight columns; even or odd rows
-  const long long col = col_base + group * 8;
   float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
   if (col < ld_e) {
-    unsigned short* column = e + row0 * ld_e + col;
     auto one = [&](int r, uint4 p) {
       const float f = factor[r][group >> 4], w = weight[r];
       uint32_t* word = reinterpret_cast<uint32_t*>(&p);
       uint4 low = make_uint4(0u, 0u, 0u, 0u);
-      if (bias_partial && w != 0.f) low = __ldcs(reinterpret_cast<const uint4*>(e_low + (row0 + r) * ld_e + col));
+      if (BIAS && w != 0.f) low = __ldcs(reinterpret_cast<const uint4*>(e_low + (row0 + r) * ld_e + col));
       const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
       const int t = target[r] - group * 8;
 #pragma unroll
@@ -1011,7 +1019,7 @@ __global__ void __launch_bounds__(256)
         float2 x = unpack2<FP16>(word[j]);
         const float2 y = unpack2<FP16>(lw[j]);
         const float h0 = t == 2 * j ? kProbScale<FP16> * w : 0.f, h1 = t == 2 * j + 1 ? kProbScale<FP16> * w : 0.f;
-        if (bias_partial && w != 0.f) {
+        if (BIAS && w != 0.f) {
           acc[2 * j] += (x.x + y.x) * f - h0;
           acc[2 * j + 1] += (x.y + y.y) * f - h1;
         }
@@ -1019,17 +1027,14 @@ __global__ void __launch_bounds__(256)
       }
       return w != 0.f ? p : make_uint4(0u, 0u, 0u, 0u);
     };
-    int r = part;
-    for (; r + 6 < n_rows; r += 8) {  // four rows at once: their loads are under way together
-      uint4 p[4];
+    for (int r0 = part; r0 < n_rows; r0 += 8) {
+      if (r0 != part) fetch(r0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const uint4*>(column + (r + 2 * i) * ld_e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(column + (r + 2 * i) * ld_e) = one(r + 2 * i, p[i]);
+      for (int i = 0; i < 4; ++i)
+        if (r0 + 2 * i < n_rows) *reinterpret_cast<uint4*>(column + (r0 + 2 * i) * ld_e) = one(r0 + 2 * i, p[i]);
     }
-    for (; r < n_rows; r += 2) *reinterpret_cast<uint4*>(column + r * ld_e) = one(r, *reinterpret_cast<const uint4*>(column + r * ld_e));
   }
-  if (bias_partial) {
+  if constexpr (BIAS) {
     if (part == 1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) sums[group][j] = acc[j];
@@ -1404,7 +1409,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     const int row_blocks = (int)((n + block_rows - 1) / block_rows);
     const bool sum_here = last && !per_row;
     EVOX_CUDA(launch_overlapped(
-        xent_rescale_kernel<FP16>, dim3((unsigned)row_blocks, (unsigned)(column_blocks + (sum_here ? 2 : dw ? 1 : 0))), 256, 0, 1, x.stream, b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss && per_row ? grad_loss + r0 : nullptr,
+        db ? xent_rescale_kernel<FP16, true> : xent_rescale_kernel<FP16, false>, dim3((unsigned)row_blocks, (unsigned)(column_blocks + (sum_here ? 2 : dw ? 1 : 0))), 256, 0, 1, x.stream, b.e, b.e_low, ld_e, b.stats, chunk, slices, b.norm, x.labels + r0, x.ignore_index, grad_loss && per_row ? grad_loss + r0 : nullptr,
         per_row, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, dw ? b.h_copy : nullptr, ld_copy,
         column_blocks, row_loss, x.rows, sum_here ? loss : nullptr));
     Join join_dh = {}, join_dw = {};
