@@ -47,29 +47,42 @@ constexpr uint32_t kSmemBytes = kOffBars + 256;  // 229,632 B of the 232,448 B a
 // 16 bits left, kOut the product itself.
 enum { kLoss = 0, kProb = 1, kOut = 2, kProbLow = 3 };
 
-struct ProductArgs {
+// One product D = A B^T over the reduction index, as tiles of 256 x 256.
+struct Product {
   long long M, N;
   int k_blocks;            // of BK
   int splits;              // the reduction is divided among this many work items per tile (kOut)
-  int chunks;              // accumulators that a tile's reduction is divided among (all but kOut)
   int tiles_m, tiles_n;
-  uint32_t stage_bytes;    // what the copies of a stage bring to both CTAs
   int m_fast, group;       // tiles run through `group` of the one direction, then all of the other
   uint32_t idesc;
+  int a_mn;                // A is contiguous along its own rows instead of the reduction (kOut)
+  // kOut: D, scaled
+  void* out16;             // [M][N], 16 bits, dense (final), or null
+  float* out32;            // [splits][M][ld32] partial sums, or the running sum over row chunks, or null
+  long long ld32;
+  int tiled_out;           // out16 has a tensor map (rows on 16-byte boundaries)
+  int add32;               // add what out32 holds before storing (or to out16)
+};
+// kOut does two products in one launch, dh and dw, so that neither waits for the other's last tiles: CTA pair q takes items
+// q, q + pairs, ... of the first, then some of the second's: the first `heavy` pairs, which have one item more of the first
+// product, `per_heavy` of them, the others `early` more before that. Neighbouring items run at the same time, so
+// that the operand lines they share are read from memory once.
+struct ProductArgs {
+  Product p[2];
+  int pairs, heavy, items[2], per_heavy, early;
+  int chunks;              // accumulators that a tile's reduction is divided among (all but kOut)
+  uint32_t stage_bytes;    // what the copies of a stage bring to both CTAs
   int* error_flag;
+  const float* scale;      // device scalar (kOut)
   // all but kOut
   const float* bias;       // [N] or null
   const long long* labels; // [M]
   float2* stats;           // [slices][ld_stats]: (maximum, sum of exponentials)
   long long ld_stats;
   float* label_logit;      // [M]
-  // kOut
-  void* out16;             // [M][ld_out] (final), or null
-  float* out32;            // [splits][M][ld32] partial sums, or the running sum over row chunks, or null
-  long long ld_out, ld32;
-  int tiled_out;           // out16 has a tensor map (rows on 16-byte boundaries)
-  int add32;               // add what out32 holds before storing (or to out16)
-  const float* scale;      // device scalar
+};
+struct Maps {
+  CUtensorMap a[2], b[2], out[2];  // of the two products; of kProb and kProbLow: out = e and what its rounding left
 };
 
 template <bool FP16>
@@ -148,29 +161,39 @@ __device__ __forceinline__ unsigned long long umma_desc_mn(uint32_t smem_addr) {
   return umma_desc(smem_addr) | ((unsigned long long)((64u * 128u) >> 4) << 16);
 }
 
-struct Tile {
-  int m, n, split;
+struct Item {
+  int which;               // product
+  int m, n;                // tile
+  int split, kb0, kb1;     // blocks of the reduction
 };
-__device__ __forceinline__ Tile tile_of(const ProductArgs& a, long long work) {
-  const long long tiles = (long long)a.tiles_m * a.tiles_n;
-  Tile t;
-  t.split = (int)(work / tiles);
-  const long long r = work - (long long)t.split * tiles;
-  const int fast = a.m_fast ? a.tiles_m : a.tiles_n, slow = a.m_fast ? a.tiles_n : a.tiles_m;
-  const int first = (int)(r / ((long long)a.group * slow)) * a.group;
-  const int width = min(a.group, fast - first);
-  const long long q = r - (long long)first * slow;
-  const int s = (int)(q / width), f = first + (int)(q - (long long)s * width);
-  t.m = a.m_fast ? f : s;
-  t.n = a.m_fast ? s : f;
+// In 32 bits (the host refuses more work items): one thread computes this between two tiles' instructions.
+__device__ __forceinline__ Item item_of(const Product& a, int which, unsigned work) {
+  const unsigned tiles = (unsigned)a.tiles_m * (unsigned)a.tiles_n;
+  Item t;
+  t.which = which;
+  unsigned r = work;
+  t.split = 0;
+  t.kb0 = 0;
+  t.kb1 = a.k_blocks;
+  if (a.splits > 1) {
+    t.split = (int)(work / tiles);
+    r = work - (unsigned)t.split * tiles;
+    const unsigned each = (unsigned)a.k_blocks / (unsigned)a.splits, more = (unsigned)a.k_blocks - each * (unsigned)a.splits;
+    t.kb0 = (int)(t.split * each + min((unsigned)t.split, more));  // the first `more` splits have a block more
+    t.kb1 = t.kb0 + (int)(each + ((unsigned)t.split < more ? 1u : 0u));
+  }
+  const unsigned fast = a.m_fast ? a.tiles_m : a.tiles_n, slow = a.m_fast ? a.tiles_n : a.tiles_m;
+  const unsigned first = r / ((unsigned)a.group * slow) * (unsigned)a.group;
+  const unsigned width = min((unsigned)a.group, fast - first);
+  const unsigned q = r - first * slow, s = q / width, f = first + (q - s * width);
+  t.m = (int)(a.m_fast ? f : s);
+  t.n = (int)(a.m_fast ? s : f);
   return t;
 }
 
-// D = A B^T over the reduction index; A_MN / B_MN: that operand is contiguous along its own rows instead.
-template <int MODE, bool A_MN, bool B_MN, bool FP16>
-__global__ void __launch_bounds__(kThreads, 1)
-    xent_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                        const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_low, const ProductArgs a) {
+// The products of ProductArgs; in kOut B is contiguous along its own rows, elsewhere both operands along the reduction.
+template <int MODE, bool FP16>
+__global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_constant__ Maps maps, const ProductArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw);
   if ((smem_base & 1023u) != 0) {  // the swizzled tiles need a 1024-byte aligned window: refuse to run otherwise
@@ -187,15 +210,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta_rank = cluster_rank();
-  const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
-  const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
-  // a tile's reduction goes to `splits` work items, or through `chunks` accumulators one after the other
-  const int chunks = MODE == kOut ? 1 : a.chunks;
-  auto kb_range = [&](int split, int chunk, int& kb0, int& kb1) {
-    const long long part = MODE == kOut ? split : chunk, parts = MODE == kOut ? a.splits : a.chunks;
-    kb0 = (int)(part * a.k_blocks / parts);
-    kb1 = (int)((part + 1) * a.k_blocks / parts);
+  // this pair's work: `count0` items of the first product, then `count1` of the second
+  const int pair = blockIdx.x >> 1;
+  const int count0 = a.items[0] > pair ? (a.items[0] - pair - 1) / a.pairs + 1 : 0;
+  const int early = pair < a.heavy ? 0 : a.early;
+  auto second = [&](int j) {  // its j-th item of the second product
+    if (j < early) return j * (a.pairs - a.heavy) + pair - a.heavy;
+    return a.early * (a.pairs - a.heavy) + (j - early) * a.pairs + pair;
   };
+  int count1 = MODE == kOut ? early + a.per_heavy : 0;
+  while (count1 > 0 && second(count1 - 1) >= a.items[1]) --count1;
+  const int n_items = count0 + count1;
+  auto item = [&](int i) {
+    if (MODE != kOut || i < count0) return item_of(a.p[0], 0, (unsigned)(pair + i * a.pairs));
+    return item_of(a.p[1], 1, (unsigned)second(i - count0));
+  };
+  const int chunks = MODE == kOut ? 1 : a.chunks;  // a tile's reduction goes through these accumulators one after the other
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -226,12 +256,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0, issued = 0;
       bool ok = true;
       const uint32_t leader_full0 = map_to_cta(full_bar(0), 0u);
-      for (long long work = first; work < n_work && ok; work += step) {
-        const Tile t = tile_of(a, work);
+      for (int i = 0; i < n_items && ok; ++i) {
+        const Item t = item(i);
         const int m0 = t.m * TM + (int)cta_rank * 128, n0 = t.n * TN + (int)cta_rank * 128;
-        const int kb0 = MODE == kOut ? (int)((long long)t.split * a.k_blocks / a.splits) : 0;
-        const int kb1 = MODE == kOut ? (int)((long long)(t.split + 1) * a.k_blocks / a.splits) : a.k_blocks;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const bool a_mn = MODE == kOut && a.p[t.which].a_mn;
+        const CUtensorMap *map_a = &maps.a[t.which], *map_b = &maps.b[t.which];
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, a.error_flag, 1)) {
             ok = false;
             break;
@@ -239,17 +269,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (cta_rank == 0) mbar_expect_tx(full_bar(s), a.stage_bytes);
           const uint32_t fb = leader_full0 + 8u * s, sa = smem_base + s * kStageBytes, sb = sa + kOperandBytes;
           const int k0 = kb * BK;
-          if constexpr (A_MN) {
-            tma_load_2d_pair(sa, &map_a, fb, m0, k0);
-            tma_load_2d_pair(sa + kOperandBytes / 2, &map_a, fb, m0 + 64, k0);
+          if (a_mn) {
+            tma_load_2d_pair(sa, map_a, fb, m0, k0);
+            tma_load_2d_pair(sa + kOperandBytes / 2, map_a, fb, m0 + 64, k0);
           } else if (cta_rank == 0 || a.stage_bytes == 2 * kStageBytes) {
-            tma_load_2d_pair(sa, &map_a, fb, k0, m0);
+            tma_load_2d_pair(sa, map_a, fb, k0, m0);
           }
-          if constexpr (B_MN) {
-            tma_load_2d_pair(sb, &map_b, fb, n0, k0);
-            tma_load_2d_pair(sb + kOperandBytes / 2, &map_b, fb, n0 + 64, k0);
+          if constexpr (MODE == kOut) {
+            tma_load_2d_pair(sb, map_b, fb, n0, k0);
+            tma_load_2d_pair(sb + kOperandBytes / 2, map_b, fb, n0 + 64, k0);
           } else {
-            tma_load_2d_pair(sb, &map_b, fb, k0, n0);
+            tma_load_2d_pair(sb, map_b, fb, k0, n0);
           }
           issued |= 1u << s;
           if (++s == STAGES) {
@@ -291,11 +321,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0;
       long long it = 0;
       bool ok = true;
-      for (long long work = first; work < n_work && ok; work += step) {
-        const Tile t = tile_of(a, work);
+      Item next = item(0);
+      for (int i = 0; i < n_items && ok; ++i) {
+        const Item t = next;
+        const bool a_mn = MODE == kOut && a.p[t.which].a_mn;
+        const uint32_t idesc = a.p[t.which].idesc;
         for (int chunk = 0; chunk < chunks && ok; ++chunk, ++it) {
-          int kb0, kb1;
-          kb_range(t.split, chunk, kb0, kb1);
+          const int kb0 = t.kb0 + chunk * kChunkBlocks, kb1 = chunk + 1 < chunks ? kb0 + kChunkBlocks : t.kb1;
           const int buf = (int)(it & 1);
           if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) {
             ok = false;
@@ -313,11 +345,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k) {
               // 16 reduction indices further: 32 bytes along a K-major line, 16 lines of an MN-major tile
-              const unsigned long long da = A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32);
-              const unsigned long long db = B_MN ? umma_desc_mn(sb + k * 2048) : umma_desc(sb + k * 32);
-              umma_f16_pair(d_tmem, da, db, a.idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+              const unsigned long long da = a_mn ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32);
+              const unsigned long long db = MODE == kOut ? umma_desc_mn(sb + k * 2048) : umma_desc(sb + k * 32);
+              umma_f16_pair(d_tmem, da, db, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
             }
             umma_commit_pair(empty_bar(s));  // stage reusable in both CTAs once these products have read it
+            if (kb == t.kb0 && i + 1 < n_items) next = item(i + 1);  // while these run
             if (++s == STAGES) {
               s = 0;
               ph ^= 1u;
@@ -334,12 +367,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t leader_tempty0 = map_to_cta(tempty_bar(0), 0u);
     uint8_t* out = smem_raw + kOffOut + (warp - 2) * kOutBytes;
     long long it = 0;
-    for (long long work = first; work < n_work; work += step) {
-      const Tile t = tile_of(a, work);
+    for (int i = 0; i < n_items; ++i) {
+      const Item t = item(i);
+      const Product& p = a.p[MODE == kOut ? t.which : 0];
       const long long row = (long long)t.m * TM + cta_rank * 128 + quarter * 32 + lane;
       const long long col0 = (long long)t.n * TN + half * kSlice;
-      const bool live = row < a.M;
-      const int width = (int)max(0ll, min((long long)kSlice, a.N - col0));  // columns of this slice that exist
+      const bool live = row < p.M;
+      const int width = (int)max(0ll, min((long long)kSlice, p.N - col0));  // columns of this slice that exist
       long long label = -1;  // column of the slice, if it is there
       if constexpr (MODE != kOut) {
         if (live) label = __ldg(a.labels + row) - col0;  // on its way while the accumulator fills
@@ -378,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ready) break;
       if constexpr (MODE == kOut) {
         const float scale = a.scale ? __ldg(a.scale) : 1.0f;
-        float* o32 = a.out32 ? a.out32 + ((long long)t.split * a.M + row) * a.ld32 + col0 : nullptr;
+        float* o32 = p.out32 ? p.out32 + ((long long)t.split * p.M + row) * p.ld32 + col0 : nullptr;
         if (o32 && live) {  // rows of out32 hold a multiple of eight columns
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -388,35 +422,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = z[c][j + i] * scale;
-                if (a.add32) {
+                if (p.add32) {
 #pragma unroll
                   for (int i = 0; i < 8; ++i) v[i] += o32[c * 32 + j + i];
                 }
-                if (!a.out16) store_32_bytes(o32 + c * 32 + j, v);
+                if (!p.out16) store_32_bytes(o32 + c * 32 + j, v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[c][j + i] = v[i];
               }
             }
         }
-        if (a.out16) {
+        if (p.out16) {
           const long long row0 = row - lane;
           const float s16 = o32 ? 1.0f : scale;
 #pragma unroll
           for (int half64 = 0; half64 < 2; ++half64) {
-            if (half64 * 64 >= width || row0 >= a.M) break;
+            if (half64 * 64 >= width || row0 >= p.M) break;
             wait_sent(lane);
             put_row<FP16>(out, lane, z[2 * half64], z[2 * half64 + 1], s16);
-            if (a.tiled_out) {
-              send_rows(&map_out, out, lane, (int)col0 + half64 * 64, (int)row0);
+            if (p.tiled_out) {
+              send_rows(&maps.out[t.which], out, lane, (int)col0 + half64 * 64, (int)row0);
             } else {  // rows that start anywhere: row by row, lanes along it
               __syncwarp();
-              unsigned short* to = reinterpret_cast<unsigned short*>(a.out16) + row0 * a.ld_out + col0 + half64 * 64;
-              const int rows_here = (int)min(32ll, a.M - row0);
+              unsigned short* to = reinterpret_cast<unsigned short*>(p.out16) + row0 * p.N + col0 + half64 * 64;
+              const int rows_here = (int)min(32ll, p.M - row0);
               for (int i = 0; i < rows_here; ++i)
 #pragma unroll
                 for (int c = lane; c < 64; c += 32)
                   if (half64 * 64 + c < width)
-                    to[i * a.ld_out + c] = *reinterpret_cast<const unsigned short*>(out + out_place(i, c >> 3) + (c & 7) * 2);
+                    to[i * p.N + c] = *reinterpret_cast<const unsigned short*>(out + out_place(i, c >> 3) + (c & 7) * 2);
             }
           }
         }
@@ -469,14 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const long long row0 = row - lane;
 #pragma unroll
           for (int half64 = 0; half64 < 2; ++half64) {
-            if (half64 * 64 >= width || row0 >= a.M) break;
+            if (half64 * 64 >= width || row0 >= p.M) break;
             wait_sent(lane);
             put_row<FP16, MODE == kProbLow>(out, lane, z[2 * half64], z[2 * half64 + 1], kProbScale<FP16>);
-            send_rows(&map_out, out, lane, (int)col0 + half64 * 64, (int)row0);
+            send_rows(&maps.out[0], out, lane, (int)col0 + half64 * 64, (int)row0);
             if constexpr (MODE == kProbLow) {
               wait_sent(lane);
               put_row<FP16>(out, lane, z[2 * half64], z[2 * half64 + 1], 1.0f);
-              send_rows(&map_low, out, lane, (int)col0 + half64 * 64, (int)row0);
+              send_rows(&maps.out[1], out, lane, (int)col0 + half64 * 64, (int)row0);
             }
           }
         }
@@ -1128,23 +1162,67 @@ int map_16(CUtensorMap* map, const void* base, long long inner, long long outer,
   return EVOX_OK;
 }
 
-template <int MODE, bool A_MN, bool B_MN, bool FP16>
-int launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_out, const CUtensorMap& map_low, ProductArgs& a,
-                   cudaStream_t stream) {
-  a.tiles_m = (int)((a.M + TM - 1) / TM);
-  a.tiles_n = (int)((a.N + TN - 1) / TN);
-  const long long n_work = (long long)a.tiles_m * a.tiles_n * a.splits;
-  const int fast = a.m_fast ? a.tiles_m : a.tiles_n;
-  if (a.group > fast) a.group = fast;
-  // fp32 accumulator, both operands of the one 16-bit type, 256 x 256; MN-major operands at bits 15 and 16
-  a.idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) |
-            (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+// fp32 accumulator, both operands of the one 16-bit type, 256 x 256; operands contiguous along their rows at bits 15 and 16.
+template <bool FP16>
+void describe(Product& p, bool a_mn, bool b_mn) {
+  p.tiles_m = (int)((p.M + TM - 1) / TM);
+  p.tiles_n = (int)((p.N + TN - 1) / TN);
+  const int fast = p.m_fast ? p.tiles_m : p.tiles_n;
+  if (p.group > fast) p.group = fast;
+  p.a_mn = a_mn;
+  p.idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) |
+            (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// Cost of a work item in blocks of the reduction; below nine blocks the epilogue is what takes the time.
+long long item_cost(const Product& p) {
+  const long long kb = (p.k_blocks + p.splits - 1) / p.splits;
+  return kb < 9 ? 9 : kb;
+}
+
+// How the work items are dealt; returns the longest pair's cost.
+long long deal(ProductArgs& a) {
+  for (int i = 0; i < 2; ++i) a.items[i] = a.p[i].M > 0 ? a.p[i].tiles_m * a.p[i].tiles_n * a.p[i].splits : 0;
+  const long long slots = sm_count() / 2, items0 = a.items[0], items1 = a.items[1];
+  const long long c0 = items0 > 0 ? item_cost(a.p[0]) : 0, c1 = items1 > 0 ? item_cost(a.p[1]) : 0;
+  a.pairs = (int)(items0 + items1 < slots ? items0 + items1 : slots);
+  a.heavy = (int)(items0 % a.pairs);
+  a.per_heavy = a.early = 0;
+  const long long light = items0 / a.pairs * c0, heavy = light + c0, fair = (items0 * c0 + items1 * c1) / a.pairs;
+  if (items1 == 0) return a.heavy ? heavy : light;
+  long long best = -1;
+  for (long long per = fair > heavy ? (fair - heavy) / c1 : 0, last = per + 1; per <= last; ++per) {  // whole items: up or down
+    const long long left = items1 - per * a.pairs, others = a.pairs - a.heavy;
+    const long long early = left > 0 ? (left + others - 1) / others : 0;
+    const long long with = a.heavy ? heavy + per * c1 : 0, without = light + (early + per) * c1, end = with > without ? with : without;
+    if (best < 0 || end < best) {
+      best = end;
+      a.per_heavy = (int)per;
+      a.early = (int)early;
+    }
+  }
+  return best;
+}
+
+template <int MODE, bool FP16>
+int launch_product(const Maps& maps, ProductArgs& a, cudaStream_t stream) {
   if (a.stage_bytes == 0) a.stage_bytes = 2 * kStageBytes;
-  const long long slots = sm_count() / 2;
-  const long long pairs = n_work < slots ? n_work : slots;
-  EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, A_MN, B_MN, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
-  EVOX_CUDA(launch_overlapped(xent_product_kernel<MODE, A_MN, B_MN, FP16>, dim3((unsigned)(2 * pairs)), kThreads, kSmemBytes, 2, stream, map_a,
-                              map_b, map_out, map_low, a));
+  if (MODE == kOut && a.p[0].M > 0 && a.p[1].M > 0) {
+    // Side by side the two products compete for the L2 cache, so they share a launch only where that saves waiting: dh and
+    // dw of 2,048 x 2,048 x 32,768 (7 % less by this count) 370 us together, 376 apart; of 8,192 x 4,096 x 131,072 (nothing
+    // to save) the whole step takes 22.8 ms together, 22.2 apart.
+    ProductArgs first = a, second = a;
+    first.p[1].M = second.p[0].M = 0;
+    const long long apart = deal(first) + deal(second), together = deal(a);
+    if (apart * 100 < together * 103) {
+      if (int rc = launch_product<MODE, FP16>(maps, first, stream)) return rc;
+      return launch_product<MODE, FP16>(maps, second, stream);
+    }
+  } else {
+    deal(a);
+  }
+  EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
+  EVOX_CUDA(launch_overlapped(xent_product_kernel<MODE, FP16>, dim3((unsigned)(2 * a.pairs)), kThreads, kSmemBytes, 2, stream, maps, a));
   return EVOX_OK;
 }
 
@@ -1155,14 +1233,21 @@ int resident_group(long long bytes_per_tile) {
   return (int)(g < 1 ? 1 : (g > 1024 ? 1024 : g));
 }
 
-// Work items per tile of a product with few tiles: enough to fill the CTA pairs, at least eight blocks of the
-// reduction each, at most 16.
-int reduction_splits(long long M, long long N, long long K) {
-  const long long tiles = ((M + TM - 1) / TM) * ((N + TN - 1) / TN), slots = sm_count() / 2, kb = (K + BK - 1) / BK;
-  long long s = slots / tiles;
-  if (s > kb / 8) s = kb / 8;
-  if (s > 16) s = 16;
-  return (int)(s < 1 ? 1 : s);
+// Into how many work items per tile the reductions of dh (rows x hidden over vocab) and dw (vocab x hidden over rows) are
+// divided: an item should not take longer than a pair's fair share of both, nor be shorter than eight blocks.
+void gradient_splits(long long rows, long long hidden, long long vocab, int& dh, int& dw) {
+  auto tiles = [](long long m, long long n) { return ((m + TM - 1) / TM) * ((n + TN - 1) / TN); };
+  const long long kb_dh = (vocab + BK - 1) / BK, kb_dw = (rows + BK - 1) / BK;
+  long long fair = (tiles(rows, hidden) * kb_dh + tiles(vocab, hidden) * kb_dw) / (sm_count() / 2);
+  if (fair < 1) fair = 1;
+  auto splits = [&](long long kb) {
+    long long s = (kb + fair - 1) / fair;
+    if (s > kb / 8) s = kb / 8;
+    if (s > 16) s = 16;
+    return (int)(s < 1 ? 1 : s);
+  };
+  dh = splits(kb_dh);
+  dw = splits(kb_dw);
 }
 
 // Rows per block of the rescaling pass: 32, or 8 where that would leave half of the machine without blocks.
@@ -1177,11 +1262,6 @@ int few_splits(long long M, long long K) {
   long long s = pairs / tiles;
   if (s > kb / 8) s = kb / 8;
   return (int)(s < 1 ? 1 : s);
-}
-
-// Splits of dh for `rows` rows.
-int dh_splits(long long rows, long long hidden, long long vocab) {
-  return rows <= kFewRows ? few_splits(hidden, vocab) : reduction_splits(rows, hidden, vocab);
 }
 
 template <int MODE, bool A_MN, bool FP16, int NT>
@@ -1248,11 +1328,14 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
     }
     b.bias_partial = with_bias ? c.take<float>(sums * vocab) : nullptr;
     size_t part_dh = 0;
+    int splits_dw = 1;
     for (long long r : {chunk, rows % chunk ? rows % chunk : chunk}) {
-      const int splits = dh_splits(r, hidden, vocab);
+      int splits;
+      gradient_splits(r, hidden, vocab, splits, splits_dw);
+      if (r <= kFewRows) splits = few_splits(hidden, vocab);
       if (splits > 1 && part_dh < (size_t)splits * r * up(hidden, 8)) part_dh = (size_t)splits * r * up(hidden, 8);
     }
-    const int splits_dw = chunk < rows ? 1 : reduction_splits(vocab, hidden, rows);
+    if (chunk < rows) splits_dw = 1;  // a running sum instead
     b.partial_dh = part_dh ? c.take<float>(part_dh) : nullptr;
     b.partial_dw = splits_dw > 1 ? c.take<float>((size_t)splits_dw * vocab * up(hidden, 8)) : nullptr;
     b.dw_sum = chunk < rows ? c.take<float>((size_t)vocab * up(hidden, 8)) : nullptr;
@@ -1266,6 +1349,8 @@ int check_operands(const char* what, const void* h, int64_t ld_h, const void* w,
   EVOX_REQUIRE(h && w && labels && loss && workspace && error_flag, EVOX_ERR_INVALID, "%s: NULL pointer", what);
   EVOX_REQUIRE(rows > 0 && hidden > 0 && vocab > 0 && rows < (1ll << 30) && hidden < (1ll << 26) && vocab < (1ll << 26), EVOX_ERR_INVALID,
                "%s: rows must be in [1, 2^30), hidden and vocab in [1, 2^26), got %lld, %lld, %lld", what, (long long)rows, (long long)hidden, (long long)vocab);
+  EVOX_REQUIRE((rows + 255) / 256 * ((vocab + 255) / 256) < (1ll << 28) && (vocab + 255) / 256 * ((hidden + 255) / 256) < (1ll << 26),
+               EVOX_ERR_INVALID, "%s: rows x vocab or vocab x hidden is too large", what);
   EVOX_REQUIRE(dtype == EVOX_DTYPE_BF16 || dtype == EVOX_DTYPE_FP16, EVOX_ERR_INVALID, "%s: operands must be bf16 or fp16", what);
   EVOX_REQUIRE(reduction == EVOX_REDUCE_NONE || reduction == EVOX_REDUCE_SUM || reduction == EVOX_REDUCE_MEAN, EVOX_ERR_INVALID,
                "%s: unknown reduction %d", what, reduction);
@@ -1299,9 +1384,9 @@ int finish(const float2* stats, long long ld_stats, const float* label_logit, co
 // Logits of `n` rows from `r0` on: (maximum, sum) per slice, the labels' logits, and the exponentials, as MODE says.
 template <int MODE, bool FP16>
 int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long long ld_stats) {
-  CUtensorMap map_a, map_b;
   const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
   if (n <= kFewRows) {
+    CUtensorMap map_a;
     if (int rc = map_16(&map_a, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
     FewArgs a = {};
     a.M = x.vocab;
@@ -1323,70 +1408,58 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
   // up to 128 rows: copies of those rows only (whole groups of eight, the swizzle's unit), none in the second CTA. Rows of a
   // tile that nothing was copied to multiply whatever is there; their products are not used.
   const int box = n <= 128 ? (int)up(n, 8) : 128;
-  if (int rc = map_16(&map_a, h, x.hidden, n, x.ld_h, box, FP16)) return rc;
-  if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
+  Maps maps;
+  if (int rc = map_16(&maps.a[0], h, x.hidden, n, x.ld_h, box, FP16)) return rc;
+  if (int rc = map_16(&maps.b[0], x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
   ProductArgs a = {};
   a.stage_bytes = n <= 128 ? 2 * kOperandBytes + (uint32_t)box * 128 : 2 * kStageBytes;
-  a.M = n;
-  a.N = x.vocab;
-  a.k_blocks = (int)((x.hidden + BK - 1) / BK);
-  a.splits = 1;
-  // a tensor-core accumulator truncates when it adds, a bias that grows with the number of additions: 1,024 hidden
-  // features per accumulator, joined with rounding (error of the mean loss at 16,384 x 4,096 x 131,072: see kChunkBlocks)
-  a.chunks = (a.k_blocks + kChunkBlocks - 1) / kChunkBlocks;
-  a.m_fast = 1;  // the weight streams past, the hidden states stay in L2
-  a.group = resident_group(2ll * TM * x.hidden);
+  Product& p = a.p[0];
+  p.M = n;
+  p.N = x.vocab;
+  p.k_blocks = (int)((x.hidden + BK - 1) / BK);
+  p.splits = 1;
+  // a tensor-core accumulator truncates when it adds, a bias that grows with the number of additions: 1,024 hidden features
+  // per accumulator, joined with rounding (mean loss at 16,384 x 4,096 x 131,072: 5.4e-7 off, 2.3e-6 with one accumulator)
+  a.chunks = (p.k_blocks + kChunkBlocks - 1) / kChunkBlocks;
+  p.m_fast = 1;  // the weight streams past, the hidden states stay in L2
+  p.group = resident_group(2ll * TM * x.hidden);
+  describe<FP16>(p, false, false);
   a.error_flag = x.error_flag;
   a.bias = x.bias;
   a.labels = x.labels + r0;
   a.stats = b.stats;
   a.ld_stats = ld_stats;
   a.label_logit = b.label_logit;
-  CUtensorMap map_e = map_a, map_low = map_a;  // not used without exponentials
+  maps.out[0] = maps.out[1] = maps.a[1] = maps.b[1] = maps.a[0];  // what this mode does not use
   if (MODE != kLoss) {
     const long long ld_e = up(x.vocab, 64);
-    if (int rc = map_16(&map_e, b.e, x.vocab, n, ld_e, 32, FP16)) return rc;
+    if (int rc = map_16(&maps.out[0], b.e, x.vocab, n, ld_e, 32, FP16)) return rc;
     if (MODE == kProbLow)
-      if (int rc = map_16(&map_low, b.e_low, x.vocab, n, ld_e, 32, FP16)) return rc;
+      if (int rc = map_16(&maps.out[1], b.e_low, x.vocab, n, ld_e, 32, FP16)) return rc;
   }
-  return launch_product<MODE, false, false, FP16>(map_a, map_b, map_e, map_low, a, x.stream);
+  return launch_product<MODE, FP16>(maps, a, x.stream);
 }
 
-// out (M x N, 16 bits, dense) = scale * A B^T with the reduction divided where that fills the machine better.
-// `sum`: running 32-bit sum over row chunks (null: this product is the whole); `first`, `last`: which chunk.
-template <bool A_MN, bool FP16>
-int gradient_product(const CUtensorMap& map_a, const CUtensorMap& map_b, long long M, long long N, long long K, int m_fast, int group,
-                     void* out, const float* scale, float* partial, float* sum, bool first, bool last, Join* join, int* error_flag,
-                     cudaStream_t stream) {
-  ProductArgs a = {};
-  a.M = M;
-  a.N = N;
-  a.k_blocks = (int)((K + BK - 1) / BK);
-  a.splits = sum ? 1 : reduction_splits(M, N, K);
-  a.m_fast = m_fast;
-  a.group = group;
-  a.error_flag = error_flag;
-  a.scale = scale;
-  a.ld_out = N;
-  a.ld32 = up(N, 8);
+// Where product `i` of `a` goes: out (M x N, 16 bits, dense), through partial sums that `join` will add up where the reduction
+// is divided, or by way of the running 32-bit sum over row chunks (`sum`; `first`, `last`: which chunk).
+template <bool FP16>
+int gradient_output(Maps& maps, ProductArgs& a, int i, void* out, float* partial, float* sum, bool first, bool last, Join* join) {
+  Product& p = a.p[i];
+  p.ld32 = up(p.N, 8);
   if (sum) {
-    a.out32 = sum;
-    a.add32 = !first;
-    a.out16 = last ? out : nullptr;
-  } else if (a.splits > 1) {
-    a.out32 = partial;
+    p.splits = 1;
+    p.out32 = sum;
+    p.add32 = !first;
+    p.out16 = last ? out : nullptr;
+  } else if (p.splits > 1) {
+    p.out32 = partial;
+    const long long blocks = (p.M * ((p.N + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
+    *join = Join{partial, reinterpret_cast<unsigned short*>(out), p.M, p.N, p.ld32, p.splits, (int)(blocks < cap ? blocks : cap)};
   } else {
-    a.out16 = out;
+    p.out16 = out;
   }
-  CUtensorMap map_out = map_a;
-  a.tiled_out = a.out16 && N % 8 == 0 && aligned16(out);
-  if (a.tiled_out)
-    if (int rc = map_16(&map_out, out, N, M, N, 32, FP16)) return rc;
-  if (int rc = launch_product<kOut, A_MN, true, FP16>(map_a, map_b, map_out, map_out, a, stream)) return rc;
-  if (a.splits > 1) {
-    const long long blocks = (M * ((N + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
-    *join = Join{partial, reinterpret_cast<unsigned short*>(out), M, N, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
-  }
+  p.tiled_out = p.out16 && p.N % 8 == 0 && aligned16(out);
+  if (p.tiled_out) return map_16(&maps.out[i], out, p.N, p.M, p.N, 32, FP16);
   return EVOX_OK;
 }
 
@@ -1413,8 +1486,10 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
         per_row, b.scalars, n, block_rows, x.vocab, db ? b.bias_partial : nullptr, h, x.ld_h, x.hidden, dw ? b.h_copy : nullptr, ld_copy,
         column_blocks, row_loss, x.rows, sum_here ? loss : nullptr));
     Join join_dh = {}, join_dw = {};
-    CUtensorMap map_a, map_b;
-    if (dh && n <= kFewRows) {
+    unsigned short* dh_rows = dh ? reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden : nullptr;
+    const bool few = n <= kFewRows;
+    if (dh && few) {
+      CUtensorMap map_a;
       if (int rc = map_16(&map_a, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
       FewArgs a = {};
       a.M = x.hidden;
@@ -1424,28 +1499,44 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
       a.error_flag = x.error_flag;
       a.scale = b.scalars;
       a.ld32 = up(x.hidden, 8);
-      unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;
       if (a.splits > 1) a.out32 = b.partial_dh;
-      else a.out16 = out;
+      else a.out16 = dh_rows;
       if (int rc = launch_few<kOut, true, FP16>(map_a, b.e, x.vocab, ld_e, a, x.stream)) return rc;
       if (a.splits > 1) {
         const long long blocks = (n * ((x.hidden + 3) / 4) + 255) / 256, cap = 16ll * sm_count();
-        join_dh = Join{b.partial_dh, out, n, x.hidden, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
+        join_dh = Join{b.partial_dh, dh_rows, n, x.hidden, a.ld32, a.splits, (int)(blocks < cap ? blocks : cap)};
       }
-    } else if (dh) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
-      if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 128, FP16)) return rc;
-      if (int rc = map_16(&map_b, x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
-      unsigned short* out = reinterpret_cast<unsigned short*>(dh) + r0 * x.hidden;
-      if (int rc = gradient_product<false, FP16>(map_a, map_b, n, x.hidden, x.vocab, 0, 8, out, b.scalars, b.partial_dh, nullptr, true, true,
-                                                 &join_dh, x.error_flag, x.stream))
-        return rc;
     }
-    if (dw) {  // g^T (contiguous along vocab) times the hidden states (contiguous along hidden)
-      if (int rc = map_16(&map_a, b.e, x.vocab, n, ld_e, 64, FP16)) return rc;
-      if (int rc = map_16(&map_b, b.h_copy, x.hidden, n, ld_copy, 64, FP16)) return rc;
-      if (int rc = gradient_product<true, FP16>(map_a, map_b, x.vocab, x.hidden, n, 0, resident_group(2ll * TN * n), dw, b.scalars,
-                                                b.partial_dw, b.dw_sum, first, last, &join_dw, x.error_flag, x.stream))
-        return rc;
+    if ((dh && !few) || dw) {
+      Maps maps;
+      ProductArgs a = {};
+      a.error_flag = x.error_flag;
+      a.scale = b.scalars;
+      gradient_splits(n, x.hidden, x.vocab, a.p[0].splits, a.p[1].splits);
+      if (int rc = map_16(&maps.a[0], b.e, x.vocab, n, ld_e, 128, FP16)) return rc;
+      maps.a[1] = maps.b[0] = maps.b[1] = maps.out[0] = maps.out[1] = maps.a[0];  // what is not set below is not used
+      if (dh && !few) {  // g (rows x vocab) times w (vocab x hidden, contiguous along hidden)
+        Product& p = a.p[0];
+        p.M = n;
+        p.N = x.hidden;
+        p.k_blocks = (int)((x.vocab + BK - 1) / BK);
+        p.group = 8;
+        if (int rc = map_16(&maps.b[0], x.w, x.hidden, x.vocab, x.ld_w, 64, FP16)) return rc;
+        describe<FP16>(p, false, true);
+        if (int rc = gradient_output<FP16>(maps, a, 0, dh_rows, b.partial_dh, nullptr, true, true, &join_dh)) return rc;
+      }
+      if (dw) {  // g^T (contiguous along vocab) times the hidden states (contiguous along hidden)
+        Product& p = a.p[1];
+        p.M = x.vocab;
+        p.N = x.hidden;
+        p.k_blocks = (int)((n + BK - 1) / BK);
+        p.group = resident_group(2ll * TN * n);
+        if (int rc = map_16(&maps.a[1], b.e, x.vocab, n, ld_e, 64, FP16)) return rc;
+        if (int rc = map_16(&maps.b[1], b.h_copy, x.hidden, n, ld_copy, 64, FP16)) return rc;
+        describe<FP16>(p, true, true);
+        if (int rc = gradient_output<FP16>(maps, a, 1, dw, b.partial_dw, b.dw_sum, first, last, &join_dw)) return rc;
+      }
+      if (int rc = launch_product<kOut, FP16>(maps, a, x.stream)) return rc;
     }
     BiasSum bias = {};
     if (db) bias = BiasSum{b.bias_partial, db, b.scalars, x.vocab, row_blocks, !first, (int)((x.vocab + 255) / 256)};
