@@ -477,6 +477,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int buf = (int)(it & 1);
       const uint32_t acc_ph = (uint32_t)((it >> 1) & 1);
       if (ok && !mbar_wait(tfull_bar(buf), acc_ph, a.error_flag, 4)) ok = false;
+      if constexpr (EPI == 3) ok = __all_sync(0xffffffffu, ok);  // the warp meets again below
       if (!ok) continue;  // keep the named barriers balanced, skip the work
       fence_after_sync();
       const float* bf = bfac + (size_t)my_ind * BN * RANK;

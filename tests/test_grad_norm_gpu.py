@@ -66,6 +66,22 @@ def test_large_and_mixed(cuda):
 
 
 @gpu
+def test_more_elements_than_32_bits_count(cuda):
+    n = 2**31 + 77
+    flat = torch.empty(n + 1, dtype=torch.bfloat16, device=cuda).normal_(generator=torch.Generator(device="cuda").manual_seed(0))
+    from evox_b200.grad_kernels import clip_grad_norm_
+
+    tail = flat[-100:].double()
+    head = flat[:100].double()
+    want = float(torch.sqrt(sum(c.float().square().sum(dtype=torch.float64) for c in flat[1:].split(2**27))))
+    norm = float(clip_grad_norm_(flat[1:], 1.0))
+    assert abs(norm - want) <= 2.0**-20 * want
+    f = 1.0 / (norm + 1e-6)
+    assert bool(((flat[-100:].double() - tail * f).abs() <= (tail * f).abs() * 2.0**-7.9 + 1e-40).all())
+    assert bool(((flat[1:100].double() - head[1:] * f).abs() <= (head[1:] * f).abs() * 2.0**-7.9 + 1e-40).all()) and float(flat[0]) == float(head[0])
+
+
+@gpu
 @pytest.mark.parametrize("scale", [1e-30, 1e-22, 1e-15, 1e15, 1e22, 3e30])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_squares_outside_the_range_of_32_bits(cuda, dtype, scale):

@@ -379,6 +379,36 @@ def test_backward_in_a_graph(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [16, 130])
+def test_offsets_beyond_32_bits(cuda, rows):
+    """A weight of more than 2^31 elements; words on both sides of that are checked in 64 bits, the normaliser comes from
+    32-bit products of every word (their error, about 2^-24 sqrt(4096) of a logit near 1, is far below the bounds used)."""
+    from evox_b200.loss_kernels import linear_cross_entropy_grad
+
+    hidden, vocab = 4096, 530_001
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(vocab, hidden, dtype=torch.bfloat16, device=cuda).normal_(0.0, 1 / 64, generator=g)
+    h = torch.randn(rows, hidden, generator=g, device=cuda).bfloat16()
+    labels = torch.randint(0, vocab, (rows,), generator=g, device=cuda)
+    labels[0], labels[1] = vocab - 1, 524_289
+    loss, dh, dw, _ = linear_cross_entropy_grad(h, w, labels, reduction="none")
+    parts = [torch.logsumexp((h.float() @ w[i : i + 65536].float().t()).double(), dim=1) for i in range(0, vocab, 65536)]
+    lse = torch.logsumexp(torch.stack(parts), dim=0)
+    want = lse - (h.double() * w[labels].double()).sum(dim=1)
+    assert float((loss.double() - want).abs().max()) <= 1e-4
+    words = torch.cat([torch.tensor([0, 524_287, 524_288, 524_289, vocab - 2, vocab - 1], device=cuda), labels])
+    p = torch.exp(h.double() @ w[words].double().t() - lse[:, None]) - (labels[:, None] == words[None, :]).double()
+    near(dw[words], p.t() @ h.double(), (p.abs().t() @ h.double().abs()) * 2.0**-6 + 1e-30, "dw")
+    del dw
+    back = -w[labels].double()
+    for i in range(0, vocab, 65536):
+        piece = w[i : i + 65536].float()
+        back += (torch.exp((h.float() @ piece.t()) - lse[:, None].float()) @ piece).double()
+    size = torch.exp(h.float() @ w[:65536].float().t() - lse[:, None].float()) @ w[:65536].float().abs() * (vocab / 65536 * 1.5) + w[labels].abs().float()
+    near(dh, back, size.double() * 2.0**-6, "dh")
+
+
+@gpu
 def test_no_wait_expired_and_a_status_is_reported_once(cuda):
     from evox_b200._cabi import EvoxKernelError
     from evox_b200.lora_kernels import raise_on_kernel_errors, status_word
@@ -418,7 +448,7 @@ def test_c_entry_refuses_bad_arguments():
         return lib.evox_linear_cross_entropy(*{**good, **kw}.values())
 
     for kw in (dict(h=None), dict(labels=None), dict(loss=None), dict(ws=None), dict(err=None), dict(rows=0), dict(rows=-1), dict(hidden=0),
-               dict(vocab=0), dict(vocab=1 << 40), dict(dtype=2), dict(reduction=3), dict(ld_h=60), dict(ld_w=56), dict(ld_w=68), dict(h=264),
+               dict(vocab=0), dict(vocab=1 << 40), dict(rows=1 << 29, vocab=1 << 25), dict(dtype=2), dict(reduction=3), dict(ld_h=60), dict(ld_w=56), dict(ld_w=68), dict(h=264),
                dict(ws=128)):
         assert call(**kw) == -1, kw
         assert b"linear_cross_entropy" in lib.evox_last_error()
