@@ -215,7 +215,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   }
 }
 
-constexpr int kSmall = 96, kLarge = 1500;  // tensors per launch: 2 KB or 30 KB of arguments (32,764 bytes are the limit)
+// Tensors per launch: 2, 8 or 30 KB of arguments (32,764 bytes are the limit); a launch pays for copying what it carries (301
+// tensors: 122 us a call with 30 KB, see clip_grad_norm_ for the rest of it).
+constexpr int kSmall = 96, kMiddle = 400, kLarge = 1500;
 
 struct Batch {
   int first, count, grid;
@@ -335,8 +337,9 @@ extern "C" int evox_clip_grad_norm(const uint64_t* address, const int64_t* numel
   int first = 0;
   do {  // once at least: the norm of nothing is 0
     const Batch b = batch_at(first);
-    if (int rc = b.count <= kSmall ? launch_square<kSmall>(b, address, numel, dtype, chunk_bytes, partial + n_partial, s)
-                                   : launch_square<kLarge>(b, address, numel, dtype, chunk_bytes, partial + n_partial, s))
+    if (int rc = b.count <= kSmall    ? launch_square<kSmall>(b, address, numel, dtype, chunk_bytes, partial + n_partial, s)
+                 : b.count <= kMiddle ? launch_square<kMiddle>(b, address, numel, dtype, chunk_bytes, partial + n_partial, s)
+                                      : launch_square<kLarge>(b, address, numel, dtype, chunk_bytes, partial + n_partial, s))
       return rc;
     n_partial += b.grid;
     first += b.count;
@@ -348,8 +351,10 @@ extern "C" int evox_clip_grad_norm(const uint64_t* address, const int64_t* numel
   first = 0;
   do {
     const Batch b = batch_at(first);
-    if (int rc = b.count <= kSmall ? launch_scale<kSmall>(b, address, numel, dtype, chunk_bytes, partial, n_partial, max_norm, first == 0, norm, s)
-                                   : launch_scale<kLarge>(b, address, numel, dtype, chunk_bytes, partial, n_partial, max_norm, first == 0, norm, s))
+    const int write_norm = first == 0;
+    if (int rc = b.count <= kSmall    ? launch_scale<kSmall>(b, address, numel, dtype, chunk_bytes, partial, n_partial, max_norm, write_norm, norm, s)
+                 : b.count <= kMiddle ? launch_scale<kMiddle>(b, address, numel, dtype, chunk_bytes, partial, n_partial, max_norm, write_norm, norm, s)
+                                      : launch_scale<kLarge>(b, address, numel, dtype, chunk_bytes, partial, n_partial, max_norm, write_norm, norm, s))
       return rc;
     first += b.count;
   } while (first < n_tensors);

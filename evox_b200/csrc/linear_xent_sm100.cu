@@ -26,6 +26,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "sm100.cuh"
 #include "xent.cuh"
 
@@ -1162,6 +1164,18 @@ int map_16(CUtensorMap* map, const void* base, long long inner, long long outer,
   return EVOX_OK;
 }
 
+// Lets a kernel use that much shared memory, once per device (bits of `allowed`; devices beyond the 64th every time).
+template <typename K>
+int allow_shared_memory(K kernel, uint32_t bytes, std::atomic<unsigned long long>& allowed) {
+  int dev = 0;
+  EVOX_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (allowed.load(std::memory_order_relaxed) & bit) return EVOX_OK;
+  EVOX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return EVOX_OK;
+}
+
 // fp32 accumulator, both operands of the one 16-bit type, 256 x 256; operands contiguous along their rows at bits 15 and 16.
 template <bool FP16>
 void describe(Product& p, bool a_mn, bool b_mn) {
@@ -1222,7 +1236,8 @@ int launch_product(const Maps& maps, ProductArgs& a, cudaStream_t stream) {
   } else {
     deal(a);
   }
-  EVOX_CUDA(cudaFuncSetAttribute(xent_product_kernel<MODE, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
+  static std::atomic<unsigned long long> allowed{0};
+  if (int rc = allow_shared_memory(xent_product_kernel<MODE, FP16>, kSmemBytes, allowed)) return rc;
   EVOX_CUDA(launch_overlapped(xent_product_kernel<MODE, FP16>, dim3((unsigned)(2 * a.pairs)), kThreads, kSmemBytes, 2, stream, maps, a));
   return EVOX_OK;
 }
@@ -1270,7 +1285,8 @@ int launch_few_nt(const CUtensorMap& map_a, const CUtensorMap& map_b, FewArgs& a
   a.tiles = (int)((a.M + 255) / 256);
   a.idesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(256 >> 4) << 24) | (FP16 ? 0u : (1u << 7) | (1u << 10)) | (A_MN ? 1u << 15 : 0u);
   const long long n_work = (long long)a.tiles * a.splits, slots = sm_count() / 2, pairs = n_work < slots ? n_work : slots;
-  EVOX_CUDA(cudaFuncSetAttribute(xent_few_kernel<MODE, A_MN, FP16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmemBytes));
+  static std::atomic<unsigned long long> allowed{0};
+  if (int rc = allow_shared_memory(xent_few_kernel<MODE, A_MN, FP16, NT>, kFewSmemBytes, allowed)) return rc;
   EVOX_CUDA(launch_overlapped(xent_few_kernel<MODE, A_MN, FP16, NT>, dim3((unsigned)(2 * pairs)), kThreads, kFewSmemBytes, 2, stream, map_a, map_b, a));
   return EVOX_OK;
 }
