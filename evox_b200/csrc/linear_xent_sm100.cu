@@ -535,11 +535,13 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
 // Few rows (up to 64). The product is bound by reading the weight once, so the operands change sides: 256 rows of the long
 // operand (the weight's, or its columns for dh) fill the tensor core's rows and the tokens are its 32 or 64 columns. A
 // block of the reduction then takes an eighth of the tensor cycles of a tile with 256 columns, and the ring holds
-// nearly nothing but the weight (ten stages). Accumulator lanes are weight rows, so the softmax statistics of a token
+// nearly nothing but the weight (ten stages). Products into one accumulator follow one another at about 160 cycles
+// however narrow they are, so the four of a block go to four accumulators. Accumulator lanes are weight rows, so the softmax statistics of a token
 // run across lanes and the four warps that share a slice of 128.
 // ---------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
-constexpr int kFewChunkBlocks = 4;  // accumulators are small and the tensor core has time: join them more often
+constexpr int kFewSums = BK / 16;       // accumulators at a time, one for each product of a block
+constexpr int kFewChunkBlocks = 16;     // blocks of the reduction that they take before they are joined
 constexpr int kFewStages = 10;
 constexpr uint32_t kFewStageBytes = kOperandBytes + 32 * 128;  // 128 lines of the long operand, up to 32 tokens' of the short one
 constexpr uint32_t kFewOffBars = kFewStages * kFewStageBytes;
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   fence_before_sync();
@@ -712,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           fence_after_sync();
-          const uint32_t d_tmem = tmem_base + (uint32_t)(buf * NT);
+          const uint32_t d_tmem = tmem_base + (uint32_t)(buf * kFewSums * NT);
           const int kb0 = chunk * count / chunks, kb1 = (chunk + 1) * count / chunks;
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
@@ -723,8 +725,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t sa = smem_base + s * kFewStageBytes, sb = sa + kOperandBytes;
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              umma_f16_pair(d_tmem, A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32), umma_desc(sb + k * 32), a.idesc,
-                            (kb > kb0 || k > 0) ? 1u : 0u);
+              umma_f16_pair(d_tmem + (uint32_t)(k * NT), A_MN ? umma_desc_mn(sa + k * 2048) : umma_desc(sa + k * 32), umma_desc(sb + k * 32),
+                            a.idesc, kb > kb0 ? 1u : 0u);
             umma_commit_pair(empty_bar(s));
             if (++s == kFewStages) {
               s = 0;
@@ -761,16 +763,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after_sync();
-        uint32_t v[T];
-        const uint32_t taddr = tmem_base + (uint32_t)(buf * NT + token0) + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t taddr = tmem_base + (uint32_t)(buf * kFewSums * NT + token0) + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-        for (int j = 0; j < T; j += 16) tmem_ld16(taddr + j, v + j);
-        tmem_ld_wait();
+        for (int k = 0; k < kFewSums; ++k) {
+          uint32_t v[T];
+#pragma unroll
+          for (int j = 0; j < T; j += 16) tmem_ld16(taddr + k * NT + j, v + j);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < T; ++j) z[j] = chunk == 0 && k == 0 ? __uint_as_float(v[j]) : z[j] + __uint_as_float(v[j]);
+        }
         fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8u * buf);
-#pragma unroll
-        for (int j = 0; j < T; ++j) z[j] = chunk == 0 ? __uint_as_float(v[j]) : z[j] + __uint_as_float(v[j]);
       }
       if constexpr (MODE == kOut) {
         if (!ok) break;
@@ -837,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // the pair leaves together
   if (warp == 1) {
     fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 128;" ::"r"(tmem_base) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
   }
 }
 
