@@ -7,7 +7,10 @@
 // table. The data are cut into equal chunks across all tensors and the chunks dealt round-robin to a fixed
 // grid, so a block's share does not depend on how the sizes are spread, and the sum is made in the same order every
 // time: no atomics. The second launch walks the chunks backwards: what the first one read last is still in the
-// L2 cache (126 MB), so gradients that fit are read from memory once.
+// L2 cache (126 MB), so gradients that fit are read from memory once. Runs of neighbouring chunks per block instead of the
+// dealing were 7 % slower.
+// Measured: 537 M fp32 values in 64 tensors 336 us for the norm (6.4 TB/s) and 1,094 us with the scaling (two reads and a
+// write, 5.9 TB/s); 50 M bf16 values in 301 tensors, which fit the L2 cache, 28 and 60 us; six tensors of 0.8 MB 4 us.
 // Sums: squares of one 16-byte vector in 32 bits, everything above in 64 bits; a vector whose squares
 // leave the safe range of 32 bits is squared again in 64 (see vector_square).
 #include <cuda_bf16.h>
@@ -215,8 +218,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   }
 }
 
-// Tensors per launch: 2, 8 or 30 KB of arguments (32,764 bytes are the limit); a launch pays for copying what it carries (301
-// tensors: 122 us a call with 30 KB, see clip_grad_norm_ for the rest of it).
+// Tensors per launch: 2, 8 or 30 KB of arguments (32,764 bytes are the limit). A launch pays for copying what it carries: both
+// launches for 301 tensors take the host 18 us with 30 KB each, 11 with 8.
 constexpr int kSmall = 96, kMiddle = 400, kLarge = 1500;
 
 struct Batch {
