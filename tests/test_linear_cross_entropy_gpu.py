@@ -68,8 +68,11 @@ class Formula:
         self.dh, self.dw, self.db = G @ w, G.t() @ hv, G.sum(dim=0)
         self.dh_tol = err @ w.abs() + (vocab / 16 + 8) * 2.0**-23 * (size @ w.abs()) + u * self.dh.abs() + tiny
         self.dw_tol = err.t() @ hv.abs() + (rows / 16 + 8) * 2.0**-23 * (size.t() @ hv.abs()) + u * self.dw.abs() + tiny
-        # the bias gradient sums 32-bit values: the exponentials with what their rounding left (off by u u)
+        # the bias gradient sums 32-bit values: the exponentials with what their rounding left (off by u u). In fp16 what is
+        # left can be subnormal: off by half of the smallest step, 2^-25, of a value that carries 2^15, so 2^-40 of c
         self.db_tol = (size * (rel - 2 * u * (1 + u) + u * u)).sum(dim=0) + (rows + 8) * 2.0**-23 * size.sum(dim=0) + 2.0**-60
+        if dtype == torch.float16:
+            self.db_tol = self.db_tol + 2.0**-40 * c.abs().sum()
 
 
 def near(got, want, tol, what):
