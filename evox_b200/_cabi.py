@@ -91,19 +91,24 @@ def ptr(t: torch.Tensor | None, dtype: torch.dtype | None = None, name: str = "t
     """Device pointer of a contiguous CUDA tensor (None passes through as NULL)."""
     if t is None:
         return None
+    device = t.get_device()  # -1 on the host
+    if device < 0 or device != torch._C._cuda_getDevice() or not t.is_contiguous() or (dtype is not None and t.dtype != dtype):
+        _refuse_tensor(t, dtype, name)
+    return t.data_ptr()
+
+
+def _refuse_tensor(t: torch.Tensor, dtype: torch.dtype | None, name: str) -> None:
     if not t.is_cuda:
         raise EvoxKernelError(f"{name} must live on a CUDA device (evox_b200 has no CPU path), got {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise EvoxKernelError(f"{name} must have dtype {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise EvoxKernelError(f"{name} must be contiguous")
-    if t.device.index != torch.cuda.current_device():
-        # the library launches on the calling thread's current device
-        raise EvoxKernelError(
-            f"{name} lives on {t.device} but the current CUDA device is cuda:{torch.cuda.current_device()}: "
-            f"make the call under `torch.cuda.device({t.device.index})` (or torch.cuda.set_device)"
-        )
-    return t.data_ptr()
+    # the library launches on the calling thread's current device
+    raise EvoxKernelError(
+        f"{name} lives on {t.device} but the current CUDA device is cuda:{torch.cuda.current_device()}: "
+        f"make the call under `torch.cuda.device({t.device.index})` (or torch.cuda.set_device)"
+    )
 
 
 def stream_ptr(device: torch.device | None = None) -> int:

@@ -74,6 +74,11 @@ def _arguments(h, weight, labels, bias, reduction):
     return h, weight, labels, bias, rest
 
 
+def _check_chunk(chunk_rows: int | None) -> None:
+    if chunk_rows is not None and chunk_rows < 1:
+        raise _cabi.EvoxKernelError(f"chunk_rows must be at least 1, got {chunk_rows}")
+
+
 def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
     dev = h.device
     rows, hidden = h.shape
@@ -124,8 +129,7 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
     (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
     are held at a time (default: all, up to 2 GiB of them)."""
     flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
-    if chunk_rows is not None and chunk_rows < 1:
-        raise _cabi.EvoxKernelError(f"chunk_rows must be at least 1, got {chunk_rows}")
+    _check_chunk(chunk_rows)
     if grad_loss is not None:
         want = shape if reduction == "none" else ()
         if grad_loss.shape != want:
@@ -142,42 +146,44 @@ class _LinearCrossEntropy(torch.autograd.Function):
     the upstream gradient; per-row losses have one upstream value per row, so theirs are computed in backward."""
 
     @staticmethod
-    def forward(ctx, h, weight, labels, bias, ignore_index, reduction):
+    def forward(ctx, h, weight, labels, bias, ignore_index, reduction, chunk_rows):
         flat, w, flat_labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
         wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
-        ctx.args = (ignore_index, reduction, shape, h.shape, None if bias is None else bias.dtype)
+        ctx.args = (ignore_index, reduction, shape, h.shape, None if bias is None else bias.dtype, chunk_rows)
         if reduction == "none":
             ctx.save_for_backward(h, weight, labels, bias)
             return _loss(flat, w, flat_labels, bias_f, ignore_index, reduction, shape)
-        loss, *grads = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape, None, None, wanted)
+        loss, *grads = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape, None, chunk_rows, wanted)
         ctx.save_for_backward(*grads)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        ignore_index, reduction, shape, h_shape, bias_dtype = ctx.args
+        ignore_index, reduction, shape, h_shape, bias_dtype, chunk_rows = ctx.args
         if reduction == "none":
             h, weight, labels, bias = ctx.saved_tensors
             flat, w, flat_labels, bias_f, _ = _arguments(h, weight, labels, bias, reduction)
             wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
             with torch.cuda.device(h.device):
                 _, dh, dw, db = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape,
-                                               grad.to(torch.float32).contiguous(), None, wanted)
+                                               grad.to(torch.float32).contiguous(), chunk_rows, wanted)
         else:
             dh, dw, db = (None if g is None else g * grad for g in ctx.saved_tensors)
-        return (None if dh is None else dh.view(h_shape), dw, None, None if db is None else db.to(bias_dtype), None, None)
+        return (None if dh is None else dh.view(h_shape), dw, None, None if db is None else db.to(bias_dtype), None, None, None)
 
 
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, bias: torch.Tensor | None = None, *,
-                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+                         ignore_index: int = -100, reduction: str = "mean", chunk_rows: int | None = None) -> torch.Tensor:
     """`F.cross_entropy(F.linear(h, weight, bias), labels)` in fp32 without the logits.
 
     `h` (..., hidden) and `weight` (vocab, hidden): both bf16 or both fp16, any sizes and row strides (rows that do not
     start on 16-byte boundaries are copied); `labels` (...) int64; `bias` (vocab,). Rows labelled `ignore_index`
     have loss 0, do not count in the mean and get zero gradients, whatever they hold; a label
     outside the vocabulary gives NaN. `reduction`: "mean", "sum" or "none" (losses shaped like `labels`).
-    Differentiable once in `h`, `weight` and `bias`."""
+    Differentiable once in `h`, `weight` and `bias`; the gradient holds 16-bit exponentials of `chunk_rows` rows at a time
+    (default: all, up to 2 GiB of them)."""
+    _check_chunk(chunk_rows)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _LinearCrossEntropy.apply(h, weight, labels, bias, ignore_index, reduction)
+        return _LinearCrossEntropy.apply(h, weight, labels, bias, ignore_index, reduction, chunk_rows)
     return _loss(*_arguments(h, weight, labels, bias, reduction)[:4], ignore_index, reduction, tuple(h.shape[:-1]))

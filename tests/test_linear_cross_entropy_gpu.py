@@ -148,7 +148,7 @@ def test_autograd_matches_the_formula(cuda, reduction):
     h, w, labels, b = make(150, 96, 333, torch.bfloat16, True)
     leaves = [t.clone().requires_grad_() for t in (h, w, b)]
     three = leaves[0].view(5, 30, 96)
-    loss = linear_cross_entropy(three, leaves[1], labels.view(5, 30), leaves[2], reduction=reduction)
+    loss = linear_cross_entropy(three, leaves[1], labels.view(5, 30), leaves[2], reduction=reduction, chunk_rows=70)
     g = torch.randn(150, generator=torch.Generator().manual_seed(3)).cuda() if reduction == "none" else torch.tensor(1.5, device=cuda)
     loss.backward(g.view(loss.shape))
     f = Formula(h, w, labels, b, reduction, g)
@@ -434,7 +434,7 @@ def test_refusals():
     h, w, y = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(9, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
     for args, kw, said in (((h, w, y), {}, "CUDA device"), ((h.float(), w.float(), y), {}, "bfloat16"), ((h, w.half(), y), {}, "bfloat16"),
                            ((h, w[:, :8], y), {}, "shape mismatch"), ((h, w[:0], y), {}, "shape mismatch"), ((h, w, y.int()), {}, "int64"),
-                           ((h, w, y[:3]), {}, "labels"), ((h, w, y, torch.zeros(8)), {}, "bias"), ((h, w, y), {"reduction": "max"}, "reduction")):
+                           ((h, w, y[:3]), {}, "labels"), ((h, w, y, torch.zeros(8)), {}, "bias"), ((h, w, y), {"reduction": "max"}, "reduction"), ((h, w, y), {"chunk_rows": 0}, "chunk_rows")):
         for fn in (linear_cross_entropy, linear_cross_entropy_grad):
             with pytest.raises(EvoxKernelError, match=said):
                 fn(*args, **kw)
