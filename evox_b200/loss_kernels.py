@@ -128,8 +128,8 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
     (`dbias` is None without a bias). Arguments as for `linear_cross_entropy`; `grad_loss` is the upstream gradient
     (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
     are held at a time (default: all, up to 2 GiB of them)."""
-    flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
     _check_chunk(chunk_rows)
+    flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
     if grad_loss is not None:
         want = shape if reduction == "none" else ()
         if grad_loss.shape != want:
