@@ -574,6 +574,7 @@ struct FewArgs {
   float* out32;            // [splits][rows][ld32], or null
   long long ld32;
   const float* scale;
+  int* tickets;            // [rows], set to 0 for the kernel that joins partial logits, or null
 };
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
@@ -653,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const uint32_t tmem_base = *((volatile uint32_t*)tmem_slot);
   overlapped_start();  // nothing of global memory was touched so far
+  if (MODE == kOut && a.tickets && blockIdx.x == 0 && (int)threadIdx.x < a.rows) a.tickets[threadIdx.x] = 0;
 
   if (warp == 0) {
     if (lane == 0) {  // TMA producer
@@ -852,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// What the rows count for, by one block of 1,024 threads (a fixed order, and the counts are whole numbers). `scalars`: [0]
+// What the rows count for, by one block (a fixed order, and the counts are whole numbers). `scalars`: [0]
 // scale of the gradient (the rows' weights are stored as fractions of the largest one, so that any upstream gradient
 // fits the 16-bit type), [1] the weights' inverse scale, [2] factor of the summed loss.
 struct Weights {
@@ -869,7 +871,7 @@ __device__ void row_weights(const Weights& a, long long ignore_index) {
   unsigned long long count = 0;
   float top = 0.f;
 #pragma unroll 4
-  for (long long i = threadIdx.x; i < a.rows; i += 1024) {
+  for (long long i = threadIdx.x; i < a.rows; i += blockDim.x) {
     const bool valid = a.labels[i] != ignore_index;
     count += valid;
     if (a.reduction == EVOX_REDUCE_NONE && a.grad_loss && valid) {
@@ -888,7 +890,7 @@ __device__ void row_weights(const Weights& a, long long ignore_index) {
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) {
+    for (int w = 1; w < (int)blockDim.x / 32; ++w) {
       count += count_part[w];
       top = fmaxf(top, max_part[w]);
     }
@@ -945,6 +947,86 @@ __global__ void __launch_bounds__(1024)
     const bool ignored = y == ignore_index, outside = !ignored && (y < 0 || y >= vocab);
     if (norm) norm[mine] = make_float2(m, outside ? NAN : 1.0f / s);
     loss[mine] = ignored ? 0.f : (outside ? NAN : (m - label_logit[mine]) + logf(s));
+  }
+}
+
+// Few rows whose logits came as partial sums over pieces of the hidden features (partial[split][row][ld]): 2,048 words of a
+// row per block; the last block of a row joins the blocks' (maximum, sum) in their order. One more block of the last grid
+// row computes the weights. A warp's first maximum may be of words past the vocabulary (-inf): rescale_to copes.
+constexpr int kJoinWords = 2048;
+__global__ void __launch_bounds__(256)
+    xent_logits_kernel(const float* __restrict__ partial, int splits, long long ld, const float* __restrict__ bias,
+                       const long long* __restrict__ labels, long long ignore_index, int rows, long long vocab, float2* parts,
+                       float* label_logit, int* tickets, float* __restrict__ loss, const Weights weights) {
+  overlapped_start();
+  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (row == rows) {
+    if (blockIdx.x == 0) row_weights(weights, ignore_index);
+    return;
+  }
+  __shared__ float sm[8], ss[8];
+  __shared__ int last;
+  const long long label = labels[row];
+  float z[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // words 4 t .. 4 t + 3 of either half of the block's
+    const long long v = (long long)blockIdx.x * kJoinWords + h * (kJoinWords / 2) + threadIdx.x * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (v < vocab) {  // lines hold a multiple of eight words
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) {
+        const float4 p = __ldcs(reinterpret_cast<const float4*>(partial + ((long long)k * rows + row) * ld + v));
+        sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+      }
+    }
+    const float got[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      z[4 * h + j] = v + j < vocab ? got[j] + (bias ? __ldg(bias + v + j) : 0.f) : -INFINITY;
+      if (v + j == label && v + j < vocab) label_logit[row] = z[4 * h + j];
+    }
+  }
+  float m = z[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = fmaxf(m, z[j]);
+  m = fmaxf(m, -INFINITY);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) sm[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, sm[w]);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += rescale_to(z[j], m);
+  s = warp_sum(s);
+  if (lane == 0) ss[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.f;
+    for (int w = 0; w < 8; ++w) s += ss[w];
+    parts[(long long)row * gridDim.x + blockIdx.x] = make_float2(m, s);
+    __threadfence();  // also of the label's logit, which another thread stored before the barriers above
+    last = atomicAdd(tickets + row, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last || warp != 0) return;
+  __threadfence();
+  m = -INFINITY;
+  s = 0.f;
+  for (int b = lane; b < (int)gridDim.x; b += 32) {
+    const float2 p = __ldcg(parts + (long long)row * gridDim.x + b);
+    const float top = fmaxf(m, p.x);
+    s = s * rescale_to(m, top) + p.y * rescale_to(p.x, top);
+    m = top;
+  }
+  const float mine = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  s = warp_sum(s * rescale_to(mine, m));
+  if (lane == 0) {
+    const bool ignored = label == ignore_index, outside = !ignored && (label < 0 || label >= vocab);
+    loss[row] = ignored ? 0.f : (outside ? NAN : (m - __ldcg(label_logit + row)) + logf(s));
   }
 }
 
@@ -1291,6 +1373,24 @@ int few_splits(long long M, long long K) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// Into how many pieces the hidden features are divided for the loss of few rows, so that the weight's tiles (256 words and
+// all features) become work items that the CTA pairs share evenly: the fewest waves of items, at 0.3 us per block of the
+// reduction, against writing and reading the partial logits at about 4 TB/s (L2 cache).
+int few_loss_splits(long long rows, long long hidden, long long vocab) {
+  const long long tiles = (vocab + 255) / 256, pairs = sm_count() / 2, kb = (hidden + BK - 1) / BK;
+  double best = 0.0;
+  int splits = 1;
+  for (int s = 1; s <= 16 && (s == 1 || kb / s >= 4); s *= 2) {
+    const double product = 0.3 * (double)((tiles * s + pairs - 1) / pairs) * (double)((kb + s - 1) / s);
+    const double cost = product + (s > 1 ? 1.0 + (double)(rows * vocab * s) * 8.0 / 4.0e6 : 0.0);
+    if (s == 1 || cost < best) {
+      best = cost;
+      splits = s;
+    }
+  }
+  return splits;
+}
+
 template <int MODE, bool A_MN, bool FP16, int NT>
 int launch_few_nt(const CUtensorMap& map_a, const CUtensorMap& map_b, FewArgs& a, cudaStream_t stream) {
   a.tiles = (int)((a.M + 255) / 256);
@@ -1334,6 +1434,9 @@ struct Buffers {
   float* bias_partial;
   float* partial_dh;  // products whose reduction is divided
   float* partial_dw;
+  float* few_logits;  // partial logits of few rows, divided features
+  float2* few_parts;
+  int* few_tickets;
   float* dw_sum;      // running dw over the row chunks
 };
 
@@ -1344,6 +1447,12 @@ size_t layout(Buffers& b, void* base, long long rows, long long hidden, long lon
   b.stats = c.take<float2>((size_t)slices * chunk);
   b.label_logit = c.take<float>(chunk);
   b.loss = c.take<float>(rows);
+  if (!grad && rows <= kFewRows) {
+    const int splits = few_loss_splits(rows, hidden, vocab);
+    b.few_logits = splits > 1 ? c.take<float>((size_t)splits * rows * up(vocab, 8)) : nullptr;
+    b.few_parts = splits > 1 ? c.take<float2>((size_t)rows * ((vocab + kJoinWords - 1) / kJoinWords)) : nullptr;
+    b.few_tickets = splits > 1 ? c.take<int>(rows) : nullptr;
+  }
   if (grad) {
     b.norm = c.take<float2>(chunk);
     b.e = c.take<unsigned short>((size_t)chunk * up(vocab, 64));
@@ -1466,6 +1575,27 @@ int logits_pass(const Head& x, const Buffers& b, long long r0, long long n, long
       if (int rc = map_16(&maps.out[1], b.e_low, x.vocab, n, ld_e, 32, FP16)) return rc;
   }
   return launch_product<MODE, FP16>(maps, a, x.stream);
+}
+
+// Losses of few rows with the features divided (few_loss_splits).
+template <bool FP16>
+int few_loss_pass(const Head& x, const Buffers& b, float* loss, const Weights& weights) {
+  CUtensorMap map_a;
+  if (int rc = map_16(&map_a, x.w, x.hidden, x.vocab, x.ld_w, 128, FP16)) return rc;
+  FewArgs a = {};
+  a.M = x.vocab;
+  a.rows = (int)x.rows;
+  a.k_blocks = (int)((x.hidden + BK - 1) / BK);
+  a.splits = few_loss_splits(x.rows, x.hidden, x.vocab);
+  a.error_flag = x.error_flag;
+  a.out32 = b.few_logits;
+  a.ld32 = up(x.vocab, 8);
+  a.tickets = b.few_tickets;
+  if (int rc = launch_few<kOut, false, FP16>(map_a, x.h, x.hidden, x.ld_h, a, x.stream)) return rc;
+  const dim3 grid((unsigned)((x.vocab + kJoinWords - 1) / kJoinWords), (unsigned)(x.rows + (weights.scalars ? 1 : 0)));
+  EVOX_CUDA(launch_overlapped(xent_logits_kernel, grid, 256, 0, 1, x.stream, b.few_logits, a.splits, a.ld32, x.bias, x.labels, x.ignore_index,
+                              a.rows, x.vocab, b.few_parts, b.label_logit, b.few_tickets, loss, weights));
+  return EVOX_OK;
 }
 
 // Where product `i` of `a` goes: out (M x N, 16 bits, dense), through partial sums that `join` will add up where the reduction
@@ -1603,10 +1733,15 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
                "linear_cross_entropy: workspace too small");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
-  if (int rc = dtype == EVOX_DTYPE_FP16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
-  const bool per_row = reduction == EVOX_REDUCE_NONE;
+  const bool per_row = reduction == EVOX_REDUCE_NONE, fp16 = dtype == EVOX_DTYPE_FP16;
   const Weights weights = {x.labels, rows, reduction, nullptr, 1.0f, per_row ? nullptr : b.scalars};
-  if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, per_row ? loss : b.loss, weights, s)) return rc;
+  float* row_loss = per_row ? loss : b.loss;
+  if (b.few_logits) {
+    if (int rc = fp16 ? few_loss_pass<true>(x, b, row_loss, weights) : few_loss_pass<false>(x, b, row_loss, weights)) return rc;
+  } else {
+    if (int rc = fp16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
+    if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, row_loss, weights, s)) return rc;
+  }
   if (!per_row) {
     EVOX_CUDA(launch_overlapped(xent_loss_sum_kernel, dim3(1), 256, 0, 1, s, b.loss, rows, b.scalars, loss));
   }

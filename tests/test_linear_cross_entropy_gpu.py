@@ -62,7 +62,8 @@ class Formula:
         G = torch.where(valid[:, None], c * (p - hot), 0.0)
         size = torch.where(valid[:, None], c.abs() * (p + hot), 0.0)
         rel = 2 * u * (1 + u) + 2 * dz[:, None] + 2.0**-20 * (zmax[:, None] + 16) + 2.0**-22
-        err = size * rel + (2.0**-38 * c.abs().max() if dtype == torch.float16 else 0.0) * valid[:, None]
+        # (an exponential below 2^-126 becomes 0)
+        err = size * rel + (2.0**-38 * c.abs().max() if dtype == torch.float16 else 2.0**-125 * c.abs().max()) * valid[:, None]
         tiny = 2.0**-25 if dtype == torch.float16 else 1e-38
         hv = torch.where(valid[:, None], h, 0.0)
         self.dh, self.dw, self.db = G @ w, G.t() @ hv, G.sum(dim=0)
@@ -83,7 +84,8 @@ def near(got, want, tol, what):
 
 SIZES = [(1, 8, 1), (1, 64, 5), (2, 1, 3), (3, 100, 257), (64, 256, 1000), (129, 512, 1009), (255, 72, 128), (256, 64, 256), (257, 1000, 1023),
          (300, 1001, 777), (1024, 256, 4099), (40, 4096, 300), (2000, 136, 70), (65, 64, 300), (128, 200, 1000), (32, 96, 129), (33, 1001, 640),
-         (9, 2200, 2500)]
+         (9, 2200, 2500), (1, 4096, 4096),
+         (33, 2048, 8000), (64, 1024, 515)]
 
 
 @gpu
