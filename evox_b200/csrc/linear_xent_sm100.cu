@@ -1237,6 +1237,35 @@ __global__ void __launch_bounds__(256) xent_loss_sum_kernel(const float* __restr
   sum_losses(loss, rows, scalars, out);
 }
 
+// Operands whose rows do not start on 16-byte boundaries (a hidden size or a stride that is no multiple of 8, an odd start)
+// are copied to rows that do, which is what TMA reads: one launch for both, eight columns per thread.
+struct Align {
+  const unsigned short* from;  // null: this operand is used as it is
+  unsigned short* to;
+  long long rows, ld_from, ld_to, cols;
+};
+__global__ void __launch_bounds__(256) xent_align_kernel(const Align h, const Align w) {
+  overlapped_start();
+  const long long n_h = h.from ? h.rows * (h.ld_to / 8) : 0, n_w = w.from ? w.rows * (w.ld_to / 8) : 0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n_h + n_w; i += (long long)gridDim.x * 256) {
+    const bool first = i < n_h;
+    const Align& a = first ? h : w;
+    const long long q = first ? i : i - n_h, r = q / (a.ld_to / 8), c = (q - r * (a.ld_to / 8)) * 8;
+    const unsigned short* src = a.from + r * a.ld_from + c;
+    uint4 p = make_uint4(0u, 0u, 0u, 0u);
+    if (c + 8 <= a.cols && (reinterpret_cast<uintptr_t>(src) & 3u) == 0) {
+      const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src);
+      p = make_uint4(__ldg(s32), __ldg(s32 + 1), __ldg(s32 + 2), __ldg(s32 + 3));
+    } else {
+      unsigned short* e = reinterpret_cast<unsigned short*>(&p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < a.cols) e[j] = __ldg(src + j);
+    }
+    *reinterpret_cast<uint4*>(a.to + r * a.ld_to + c) = p;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------------------------
@@ -1423,6 +1452,8 @@ struct Carve {  // 256-byte aligned pieces of the workspace
 };
 
 struct Buffers {
+  unsigned short* h_aligned;
+  unsigned short* w_aligned;
   float* scalars;
   float2* stats;
   float* label_logit;
@@ -1440,8 +1471,12 @@ struct Buffers {
   float* dw_sum;      // running dw over the row chunks
 };
 
-size_t layout(Buffers& b, void* base, long long rows, long long hidden, long long vocab, long long chunk, bool grad, bool with_bias) {
+// copies: bit 0: the hidden states are copied to aligned rows, bit 1: the weight is.
+size_t layout(Buffers& b, void* base, long long rows, long long hidden, long long vocab, int copies, long long chunk, bool grad,
+              bool with_bias) {
   Carve c{reinterpret_cast<uint8_t*>(base), 0};
+  b.h_aligned = copies & 1 ? c.take<unsigned short>((size_t)rows * up(hidden, 8)) : nullptr;
+  b.w_aligned = copies & 2 ? c.take<unsigned short>((size_t)vocab * up(hidden, 8)) : nullptr;
   const long long slices = (vocab + kSlice - 1) / kSlice;
   b.scalars = c.take<float>(4);
   b.stats = c.take<float2>((size_t)slices * chunk);
@@ -1491,11 +1526,14 @@ int check_operands(const char* what, const void* h, int64_t ld_h, const void* w,
   EVOX_REQUIRE(dtype == EVOX_DTYPE_BF16 || dtype == EVOX_DTYPE_FP16, EVOX_ERR_INVALID, "%s: operands must be bf16 or fp16", what);
   EVOX_REQUIRE(reduction == EVOX_REDUCE_NONE || reduction == EVOX_REDUCE_SUM || reduction == EVOX_REDUCE_MEAN, EVOX_ERR_INVALID,
                "%s: unknown reduction %d", what, reduction);
-  EVOX_REQUIRE(ld_h >= hidden && ld_w >= hidden && ld_h % 8 == 0 && ld_w % 8 == 0, EVOX_ERR_INVALID,
-               "%s: row strides must be multiples of 8 elements and at least hidden", what);
-  EVOX_REQUIRE(aligned16(h) && aligned16(w), EVOX_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
+  EVOX_REQUIRE(ld_h >= hidden && ld_w >= hidden, EVOX_ERR_INVALID, "%s: row strides must be at least hidden", what);
+  EVOX_REQUIRE(((uintptr_t)h & 1u) == 0 && ((uintptr_t)w & 1u) == 0, EVOX_ERR_INVALID, "%s: operands must be aligned to their elements", what);
   EVOX_REQUIRE(((uintptr_t)workspace & 255u) == 0, EVOX_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
   return EVOX_OK;
+}
+
+int copies_of(const void* h, long long ld_h, const void* w, long long ld_w) {
+  return (aligned16(h) && ld_h % 8 == 0 ? 0 : 1) | (aligned16(w) && ld_w % 8 == 0 ? 0 : 2);
 }
 
 struct Head {
@@ -1515,6 +1553,25 @@ int finish(const float2* stats, long long ld_stats, const float* label_logit, co
   const int slices = (int)((vocab + kSlice - 1) / kSlice);
   EVOX_CUDA(launch_overlapped(xent_finish_kernel, dim3((unsigned)((rows + 31) / 32 + (weights.scalars ? 1 : 0))), 1024, 0, 1, stream, stats,
                               ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, weights));
+  return EVOX_OK;
+}
+
+// Replaces operands that TMA cannot read by aligned copies in the workspace.
+int align_operands(Head& x, const Buffers& b) {
+  if (!b.h_aligned && !b.w_aligned) return EVOX_OK;
+  const long long ld = up(x.hidden, 8);
+  const Align h = {b.h_aligned ? (const unsigned short*)x.h : nullptr, b.h_aligned, x.rows, x.ld_h, ld, x.hidden};
+  const Align w = {b.w_aligned ? (const unsigned short*)x.w : nullptr, b.w_aligned, x.vocab, x.ld_w, ld, x.hidden};
+  const long long n = ((h.from ? x.rows : 0) + (w.from ? x.vocab : 0)) * (ld / 8), blocks = (n + 255) / 256, cap = 32ll * sm_count();
+  EVOX_CUDA(launch_overlapped(xent_align_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), 256, 0, 1, x.stream, h, w));
+  if (b.h_aligned) {
+    x.h = b.h_aligned;
+    x.ld_h = ld;
+  }
+  if (b.w_aligned) {
+    x.w = b.w_aligned;
+    x.ld_w = ld;
+  }
   return EVOX_OK;
 }
 
@@ -1716,10 +1773,14 @@ int xent_finish(const float2* stats, long long ld_stats, const float* label_logi
 
 using namespace evox;
 
-extern "C" size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
+extern "C" int32_t evox_linear_cross_entropy_copies(const void* h, int64_t ld_h, const void* w, int64_t ld_w) {
+  return copies_of(h, ld_h, w, ld_w);
+}
+
+extern "C" size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab, int32_t copies) {
   if (rows <= 0 || hidden <= 0 || vocab <= 0) return 0;
   Buffers b = {};
-  return layout(b, nullptr, rows, hidden, vocab, rows, false, false);
+  return layout(b, nullptr, rows, hidden, vocab, copies, rows, false, false);
 }
 
 extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype, const float* bias,
@@ -1729,10 +1790,11 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
   if (int rc = check_operands("linear_cross_entropy", h, ld_h, w, ld_w, dtype, labels, rows, hidden, vocab, reduction, loss, workspace, error_flag))
     return rc;
   Buffers b = {};
-  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, rows, false, false), EVOX_ERR_WORKSPACE,
+  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, copies_of(h, ld_h, w, ld_w), rows, false, false), EVOX_ERR_WORKSPACE,
                "linear_cross_entropy: workspace too small");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  if (int rc = align_operands(x, b)) return rc;
   const bool per_row = reduction == EVOX_REDUCE_NONE, fp16 = dtype == EVOX_DTYPE_FP16;
   const Weights weights = {x.labels, rows, reduction, nullptr, 1.0f, per_row ? nullptr : b.scalars};
   float* row_loss = per_row ? loss : b.loss;
@@ -1757,10 +1819,10 @@ extern "C" int64_t evox_linear_cross_entropy_chunk_rows(int64_t rows, int64_t vo
 }
 
 extern "C" size_t evox_linear_cross_entropy_grad_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab, int64_t chunk_rows,
-                                                                 int32_t with_bias) {
+                                                                 int32_t with_bias, int32_t copies) {
   if (rows <= 0 || hidden <= 0 || vocab <= 0 || chunk_rows <= 0) return 0;
   Buffers b = {};
-  return layout(b, nullptr, rows, hidden, vocab, chunk_rows < rows ? chunk_rows : rows, true, with_bias != 0);
+  return layout(b, nullptr, rows, hidden, vocab, copies, chunk_rows < rows ? chunk_rows : rows, true, with_bias != 0);
 }
 
 extern "C" int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype, const float* bias,
@@ -1772,10 +1834,11 @@ extern "C" int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const
   EVOX_REQUIRE(chunk_rows > 0, EVOX_ERR_INVALID, "linear_cross_entropy_grad: chunk_rows must be positive");
   const long long chunk = chunk_rows < rows ? chunk_rows : rows;
   Buffers b = {};
-  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, chunk, true, dbias != nullptr), EVOX_ERR_WORKSPACE,
+  EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, copies_of(h, ld_h, w, ld_w), chunk, true, dbias != nullptr), EVOX_ERR_WORKSPACE,
                "linear_cross_entropy_grad: workspace too small");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  Head x = {h, ld_h, w, ld_w, bias, (const long long*)labels, ignore_index, rows, hidden, vocab, error_flag, s};
+  if (int rc = align_operands(x, b)) return rc;
   return dtype == EVOX_DTYPE_FP16 ? gradient_pass<true>(x, b, chunk, reduction, grad_loss, loss, dh, dw, dbias)
                                   : gradient_pass<false>(x, b, chunk, reduction, grad_loss, loss, dh, dw, dbias);
 }

@@ -9,7 +9,6 @@ virtual-LoRA population is `lora_kernels.lora_layer_cross_entropy`.
 from __future__ import annotations
 
 import torch
-import torch.nn.functional as F
 
 from . import _cabi
 from .lora_kernels import status_word
@@ -20,20 +19,15 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
-def _operand(x: torch.Tensor, rows: int, hidden: int) -> tuple[torch.Tensor, int]:
-    """`x` (rows, hidden) with rows that start on 16-byte boundaries, and its row stride; a view is used as it is
-    where it can be, anything else is copied."""
+def _operand(x: torch.Tensor, rows: int, hidden: int) -> tuple[torch.Tensor, int, bool]:
+    """`x` (rows, hidden) with dense rows, its row stride, and whether its rows start off 16-byte boundaries (the kernels
+    then copy it to their workspace)."""
     stride, step = x.stride()
     if rows == 1:
         stride = (hidden + 7) // 8 * 8
-    if (step == 1 or hidden == 1) and stride % 8 == 0 and stride >= hidden and x.data_ptr() % 16 == 0:
-        return x, stride
-    pad = -hidden % 8
-    with torch.no_grad():
-        x = F.pad(x, (0, pad)) if pad else x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x, hidden + pad
+    if (step != 1 and hidden != 1) or stride < hidden:
+        x, stride = x.detach().contiguous(), hidden
+    return x, stride, stride % 8 != 0 or x.data_ptr() % 16 != 0
 
 
 def _refuse(h, weight, labels, bias, reduction):
@@ -85,10 +79,10 @@ def _loss(h, weight, labels, bias, ignore_index, reduction, shape):
     vocab = weight.shape[0]
     if rows == 0:
         return torch.full(shape if reduction == "none" else (), float("nan") if reduction == "mean" else 0.0, device=dev)
-    (h, ld_h), (weight, ld_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
+    (h, ld_h, copy_h), (weight, ld_w, copy_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
     loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
     lib = _cabi.lib
-    nbytes = lib.evox_linear_cross_entropy_workspace_bytes(rows, hidden, vocab)
+    nbytes = lib.evox_linear_cross_entropy_workspace_bytes(rows, hidden, vocab, copy_h + 2 * copy_w)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _cabi.check(lib.evox_linear_cross_entropy(
         h.data_ptr(), ld_h, weight.data_ptr(), ld_w, _DTYPES[h.dtype], None if bias is None else bias.data_ptr(), labels.data_ptr(),
@@ -107,11 +101,11 @@ def _loss_and_grad(h, weight, labels, bias, ignore_index, reduction, shape, grad
     db = torch.empty(vocab, dtype=torch.float32, device=dev) if wanted[2] and bias is not None else None
     if rows == 0:
         return _loss(h, weight, labels, bias, ignore_index, reduction, shape), dh, *(None if g is None else g.zero_() for g in (dw, db))
-    (h, ld_h), (weight, ld_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
+    (h, ld_h, copy_h), (weight, ld_w, copy_w) = _operand(h, rows, hidden), _operand(weight, vocab, hidden)
     loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
     lib = _cabi.lib
     chunk = lib.evox_linear_cross_entropy_chunk_rows(rows, vocab) if chunk_rows is None else chunk_rows
-    nbytes = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, hidden, vocab, chunk, db is not None)
+    nbytes = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, hidden, vocab, chunk, db is not None, copy_h + 2 * copy_w)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _cabi.check(lib.evox_linear_cross_entropy_grad(
         h.data_ptr(), ld_h, weight.data_ptr(), ld_w, _DTYPES[dtype], None if bias is None else bias.data_ptr(), labels.data_ptr(),

@@ -577,13 +577,16 @@ int evox_bench_compare_rate(const float* in, uint32_t* out, int32_t iterations, 
 #define EVOX_REDUCE_MEAN 2 /* over the rows whose label is not ignore_index (none: NaN) */
 
 /* loss = log sum_v exp(z_v) - z_label per row, z = h w^T + bias, with h (rows x hidden, row stride
- * ld_h) and w (vocab x hidden, row stride ld_w) in bf16 or fp16, strides multiples of 8 elements and
- * 16-byte aligned bases; bias (vocab, fp32) or NULL; fp32 sums. A row whose label is ignore_index has
+ * ld_h) and w (vocab x hidden, row stride ld_w) in bf16 or fp16. Operands whose rows do not all start
+ * on 16-byte boundaries are copied to the workspace: evox_linear_cross_entropy_copies says which (bit 0:
+ * h, bit 1: w), and its answer is the argument `copies` of the workspace's size. bias (vocab, fp32) or NULL; fp32 sums. A row whose label is ignore_index has
  * loss 0; any other label outside [0, vocab) gives NaN. loss: rows values (EVOX_REDUCE_NONE) or one.
  * The logits are not stored: the workspace holds 8 bytes per row and 128 columns. error_flag: a
  * device int32 that holds 0, set to a status if a bounded device-side wait expired; one word may serve
  * any number of calls. */
-size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
+int32_t evox_linear_cross_entropy_copies(const void* h, int64_t ld_h, const void* w, int64_t ld_w);
+size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab,
+                                                 int32_t copies);
 int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_t ld_w, int32_t dtype,
                               const float* bias, const int64_t* labels, int64_t ignore_index,
                               int64_t rows, int64_t hidden, int64_t vocab, int32_t reduction,
@@ -597,7 +600,8 @@ int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_
  * Python wrapper uses (at most 2 GiB of them). with_bias: whether dbias will be given. */
 int64_t evox_linear_cross_entropy_chunk_rows(int64_t rows, int64_t vocab);
 size_t evox_linear_cross_entropy_grad_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab,
-                                                      int64_t chunk_rows, int32_t with_bias);
+                                                      int64_t chunk_rows, int32_t with_bias,
+                                                      int32_t copies);
 int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const void* w, int64_t ld_w,
                                    int32_t dtype, const float* bias, const int64_t* labels,
                                    int64_t ignore_index, int64_t rows, int64_t hidden, int64_t vocab,

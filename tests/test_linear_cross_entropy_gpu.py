@@ -453,13 +453,16 @@ def test_c_entry_refuses_bad_arguments():
         return lib.evox_linear_cross_entropy(*{**good, **kw}.values())
 
     for kw in (dict(h=None), dict(labels=None), dict(loss=None), dict(ws=None), dict(err=None), dict(rows=0), dict(rows=-1), dict(hidden=0),
-               dict(vocab=0), dict(vocab=1 << 40), dict(rows=1 << 29, vocab=1 << 25), dict(dtype=2), dict(reduction=3), dict(ld_h=60), dict(ld_w=56), dict(ld_w=68), dict(h=264),
+               dict(vocab=0), dict(vocab=1 << 40), dict(rows=1 << 29, vocab=1 << 25), dict(dtype=2), dict(reduction=3), dict(ld_h=60), dict(ld_w=56), dict(h=257), dict(w=259),
                dict(ws=128)):
         assert call(**kw) == -1, kw
         assert b"linear_cross_entropy" in lib.evox_last_error()
     assert call(nbytes=16) == -3
-    assert lib.evox_linear_cross_entropy_workspace_bytes(0, 4, 4) == 0
+    assert lib.evox_linear_cross_entropy_workspace_bytes(0, 4, 4, 0) == 0
+    assert [lib.evox_linear_cross_entropy_copies(*a) for a in ((256, 64, 256, 64), (258, 64, 256, 64), (256, 64, 256, 65), (264, 8, 272, 12))] == [0, 1, 2, 3]
+    plain = lib.evox_linear_cross_entropy_workspace_bytes(4, 63, 9, 0)
+    assert lib.evox_linear_cross_entropy_workspace_bytes(4, 63, 9, 1) == plain + 512 and lib.evox_linear_cross_entropy_workspace_bytes(4, 63, 9, 2) == plain + 1280
     rows, vocab = 100000, 131072
     assert lib.evox_linear_cross_entropy_chunk_rows(rows, vocab) == 8192 and lib.evox_linear_cross_entropy_chunk_rows(100, vocab) == 100
-    small = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, 64, vocab, 256, 0)
-    assert small < lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, 64, vocab, 512, 0)
+    small = lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, 64, vocab, 256, 0, 0)
+    assert small < lib.evox_linear_cross_entropy_grad_workspace_bytes(rows, 64, vocab, 512, 0, 0)
