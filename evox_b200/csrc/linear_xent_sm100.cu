@@ -1198,13 +1198,22 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const Join dh, const Joi
   overlapped_start();
   int block = blockIdx.x;
   if (block < db.blocks) {
-    const long long v = (long long)block * 256 + threadIdx.x;
-    if (v >= db.vocab) return;
+    // 32 columns, the row blocks dealt to eight warps
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long v = (long long)block * 32 + lane;
     float s = 0.f;
+    if (v < db.vocab) {
 #pragma unroll 8
-    for (int b = 0; b < db.row_blocks; ++b) s += __ldg(db.partial + (long long)b * db.vocab + v);
-    s *= db.scale[0];
-    db.out[v] = db.add ? db.out[v] + s : s;
+      for (int b = warp; b < db.row_blocks; b += 8) s += __ldg(db.partial + (long long)b * db.vocab + v);
+    }
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && v < db.vocab) {
+      for (int w = 1; w < 8; ++w) s += part[w][lane];
+      s *= db.scale[0];
+      db.out[v] = db.add ? db.out[v] + s : s;
+    }
     return;
   }
   block -= db.blocks;
@@ -1754,7 +1763,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
       if (int rc = launch_product<kOut, FP16>(maps, a, x.stream)) return rc;
     }
     BiasSum bias = {};
-    if (db) bias = BiasSum{b.bias_partial, db, b.scalars, x.vocab, row_blocks, !first, (int)((x.vocab + 255) / 256)};
+    if (db) bias = BiasSum{b.bias_partial, db, b.scalars, x.vocab, row_blocks, !first, (int)((x.vocab + 31) / 32)};
     if (const int blocks = join_dh.blocks + join_dw.blocks + bias.blocks) {
       EVOX_CUDA(launch_overlapped(xent_join_kernel<FP16>, dim3((unsigned)blocks), 256, 0, 1, x.stream, join_dh, join_dw, bias));
     }
