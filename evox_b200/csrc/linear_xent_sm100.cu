@@ -453,11 +453,21 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
               __syncwarp();
               unsigned short* to = reinterpret_cast<unsigned short*>(p.out16) + row0 * p.N + col0 + half64 * 64;
               const int rows_here = (int)min(32ll, p.M - row0);
-              for (int i = 0; i < rows_here; ++i)
+              if (p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(p.out16) & 3u) == 0) {  // pairs of columns, 128 bytes of a row at once
+                if (half64 * 64 + 2 * lane < width) {
+#pragma unroll 8
+                  for (int i = 0; i < rows_here; ++i)
+                    *reinterpret_cast<uint32_t*>(to + i * p.N + 2 * lane) =
+                        *reinterpret_cast<const uint32_t*>(out + out_place(i, lane >> 2) + (lane & 3) * 4);
+                }
+              } else {
+#pragma unroll 4
+                for (int i = 0; i < rows_here; ++i)
 #pragma unroll
-                for (int c = lane; c < 64; c += 32)
-                  if (half64 * 64 + c < width)
-                    to[i * p.N + c] = *reinterpret_cast<const unsigned short*>(out + out_place(i, c >> 3) + (c & 7) * 2);
+                  for (int c = lane; c < 64; c += 32)
+                    if (half64 * 64 + c < width)
+                      to[i * p.N + c] = *reinterpret_cast<const unsigned short*>(out + out_place(i, c >> 3) + (c & 7) * 2);
+              }
             }
           }
         }
