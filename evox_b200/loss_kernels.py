@@ -136,15 +136,17 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
-    """A scalar loss computes its gradients with the forward pass, while the exponentials are there, and scales them by
-    the upstream gradient; per-row losses have one upstream value per row, so theirs are computed in backward."""
+    """A scalar loss of bf16 operands computes its gradients with the forward pass, while the exponentials are there, and
+    backward multiplies them by the upstream gradient (in 32 bits, one more rounding to bf16). Elsewhere backward computes
+    them: per-row losses have one upstream value per row, and fp16 would lose what a loss scale is there to keep (numbers
+    below 6e-8, or above 65,504 before a small factor) if it rounded before the upstream value is applied."""
 
     @staticmethod
     def forward(ctx, h, weight, labels, bias, ignore_index, reduction, chunk_rows):
         flat, w, flat_labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
         wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
         ctx.args = (ignore_index, reduction, shape, h.shape, None if bias is None else bias.dtype, chunk_rows)
-        if reduction == "none":
+        if reduction == "none" or h.dtype == torch.float16:
             ctx.save_for_backward(h, weight, labels, bias)
             return _loss(flat, w, flat_labels, bias_f, ignore_index, reduction, shape)
         loss, *grads = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape, None, chunk_rows, wanted)
@@ -155,7 +157,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         ignore_index, reduction, shape, h_shape, bias_dtype, chunk_rows = ctx.args
-        if reduction == "none":
+        if len(ctx.saved_tensors) == 4:
             h, weight, labels, bias = ctx.saved_tensors
             flat, w, flat_labels, bias_f, _ = _arguments(h, weight, labels, bias, reduction)
             wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
@@ -163,7 +165,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 _, dh, dw, db = _loss_and_grad(flat, w, flat_labels, bias_f, ignore_index, reduction, shape,
                                                grad.to(torch.float32).contiguous(), chunk_rows, wanted)
         else:
-            dh, dw, db = (None if g is None else g * grad for g in ctx.saved_tensors)
+            # one element, not a 0-d tensor: that would be rounded to bf16 before the product
+            dh, dw, db = (None if g is None else torch.mul(g, grad.reshape(1), out=torch.empty_like(g)) for g in ctx.saved_tensors)
         return (None if dh is None else dh.view(h_shape), dw, None, None if db is None else db.to(bias_dtype), None, None, None)
 
 
