@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
     // ------------------------------- TMA producer ------------------------------------------
     if (lane == 0) {
       int s = 0;
-      uint32_t ph = 0, issued = 0;
+      uint32_t ph = 0;
       bool ok = true;
       const uint32_t leader_full0 = map_to_cta(full_bar(0), 0u);
       for (int i = 0; i < n_items && ok; ++i) {
@@ -288,7 +288,6 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
           } else {
             tma_load_2d_pair(sb, map_b, fb, k0, n0);
           }
-          issued |= 1u << s;
           if (++s == STAGES) {
             s = 0;
             ph ^= 1u;
@@ -304,22 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
           ph ^= 1u;
         }
       }
-      if (!ok) {
-        // drain: the last copy issued into each stage must land before shared memory is released; the follower's
-        // copies report to the leader, so it cannot see them
-        for (int q = 0; q < STAGES && cta_rank == 0; ++q) {
-          if (!(issued & (1u << q))) continue;
-          const uint32_t last = (q < s) ? ph : (ph ^ 1u);
-          const unsigned long long t0 = global_timer_ns();
-          while (!mbar_try(full_bar(q), last) && !mbar_try(full_bar(q), last ^ 1u)) {
-            if (global_timer_ns() - t0 > kWaitLimitNs) break;
-          }
-        }
-        // copies and products that nothing here can observe: give them a millisecond, far beyond their latency
-        const unsigned long long t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 1000000ull) {
-        }
-      }
+      if (!ok) settle();
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer --------------------------------------------
@@ -366,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
           if (ok) umma_commit_pair(tfull_bar(buf));  // accumulator complete
         }
       }
+      if (!ok) settle();
     }
   } else {
     // ------------------------------- epilogue (256 threads) --------------------------------
@@ -416,7 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8u * buf);
       }
-      if (!ready) break;
+      if (!ready) {
+        settle();
+        break;
+      }
       if constexpr (MODE == kOut) {
         const float scale = a.scale ? __ldg(a.scale) : 1.0f;
         float* o32 = p.out32 ? p.out32 + ((long long)t.split * p.M + row) * p.ld32 + col0 : nullptr;
@@ -669,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     if (lane == 0) {  // TMA producer
       int s = 0;
-      uint32_t ph = 0, issued = 0;
+      uint32_t ph = 0;
       bool ok = true;
       const uint32_t leader_full0 = map_to_cta(full_bar(0), 0u);
       for (int work = first; work < n_work && ok; work += step) {
@@ -689,7 +677,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d_pair(sa, &map_a, fb, k0, m0);
           }
           tma_load_2d_pair(sb, &map_b, fb, k0, (int)cta_rank * T);
-          issued |= 1u << s;
           if (++s == kFewStages) {
             s = 0;
             ph ^= 1u;
@@ -704,19 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ph ^= 1u;
         }
       }
-      if (!ok) {  // as in xent_product_kernel: nothing may be under way when shared memory is released
-        for (int q = 0; q < kFewStages && cta_rank == 0; ++q) {
-          if (!(issued & (1u << q))) continue;
-          const uint32_t last = (q < s) ? ph : (ph ^ 1u);
-          const unsigned long long t0 = global_timer_ns();
-          while (!mbar_try(full_bar(q), last) && !mbar_try(full_bar(q), last ^ 1u)) {
-            if (global_timer_ns() - t0 > kWaitLimitNs) break;
-          }
-        }
-        const unsigned long long t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 1000000ull) {
-        }
-      }
+      if (!ok) settle();
     }
   } else if (warp == 1) {
     if (lane == 0 && cta_rank == 0) {  // MMA issuer
@@ -754,6 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok) umma_commit_pair(tfull_bar(buf));
         }
       }
+      if (!ok) settle();
     }
   } else {
     // epilogue: lanes are rows of the long operand, warps 2-5 and 6-9 take half of the tokens each
@@ -854,6 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    if (!ok) settle();
   }
   fence_before_sync();
   __syncthreads();

@@ -26,7 +26,7 @@
 // "full" barrier; tcgen05.commit releases the stage in both CTAs and hands the accumulator to both
 // epilogues; the epilogues return accumulators to the leader's "empty" barrier by a remote arrive.
 // Every mbarrier wait is bounded by a wall-clock limit; on expiry the kernel raises an error flag,
-// all roles leave their loops, outstanding copies are drained with the same bound and TMEM is freed.
+// all roles leave their loops, what is under way gets a millisecond to end (settle) and TMEM is freed.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -221,7 +221,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
-      uint32_t issued = 0;  // bit s: a copy into stage s may still be in flight
       bool ok = true;
       const uint32_t leader_full0 = PAIR ? map_to_cta(full_bar(0), 0u) : full_bar(0);
       for (long long work = tile_first; work < n_work && ok; work += tile_step) {
@@ -247,7 +246,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tma_load_2d(smem_base + s * kStageBytes, &map_h, full_bar(s), (int)(a.a_piece[combo] * a.K) + kk * BK, m0);
             tma_load_2d(smem_base + s * kStageBytes + kBytesA, &map_w, full_bar(s), (int)(a.b_piece[combo] * a.K) + kk * BK, n0);
           }
-          issued |= 1u << s;
           if (++s == STAGES) {
             s = 0;
             ph ^= 1u;
@@ -265,26 +263,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
-      if (!ok) {
-        // drain: the last copy issued into each stage must land before shared memory is released
-        for (int q = 0; q < STAGES; ++q) {
-          if (!(issued & (1u << q))) continue;
-          if (PAIR && cta_rank != 0) continue;  // the follower's copies report to the leader: timed wait below
-          // stage q was last filled in phase (ph if q < s else ph ^ 1)
-          const uint32_t last = (q < s) ? ph : (ph ^ 1u);
-          const unsigned long long t0 = global_timer_ns();
-          while (!mbar_try(full_bar(q), last) && !mbar_try(full_bar(q), last ^ 1u)) {
-            if (global_timer_ns() - t0 > kWaitLimitNs) break;
-          }
-        }
-        if constexpr (PAIR) {
-          // nothing in this CTA can observe the follower's copies (or the products the leader still has in
-          // flight on this CTA's shared memory): give them a millisecond, far beyond their latency
-          const unsigned long long t0 = global_timer_ns();
-          while (global_timer_ns() - t0 < 1000000ull) {
-          }
-        }
-      }
+      if (!ok) settle();
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer --------------------------------------------
@@ -332,6 +311,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
+      if (!ok) settle();
     }
   } else {
     // ------------------------------- epilogue (256 threads) --------------------------------
@@ -379,6 +359,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const int buf = (int)(it & 1);
           const uint32_t acc_ph = (uint32_t)((it >> 1) & 1);
           if (ok && !mbar_wait(tfull_bar(buf), acc_ph, a.error_flag, 4)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);  // tensor memory is read by whole warps
           if (!ok) continue;
           fence_after_sync();
           const float cs = a.combo_scale[(chunk * chunk_kb) / k_blocks];  // a chunk never straddles two passes
@@ -477,7 +458,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int buf = (int)(it & 1);
       const uint32_t acc_ph = (uint32_t)((it >> 1) & 1);
       if (ok && !mbar_wait(tfull_bar(buf), acc_ph, a.error_flag, 4)) ok = false;
-      if constexpr (EPI == 3) ok = __all_sync(0xffffffffu, ok);  // the warp meets again below
+      ok = __all_sync(0xffffffffu, ok);  // tensor memory is read by whole warps
       if (!ok) continue;  // keep the named barriers balanced, skip the work
       fence_after_sync();
       const float* bf = bfac + (size_t)my_ind * BN * RANK;
@@ -591,6 +572,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if constexpr (PAIR) mbar_arrive_cluster(leader_tempty0 + 8u * buf); else mbar_arrive(tempty_bar(buf));
       }
     }
+    if (!ok) settle();
   }
   fence_before_sync();
   __syncthreads();

@@ -54,6 +54,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
   }
 }
 
+// A role whose wait gave up calls this before it leaves: copies and products already under way must be over before shared
+// and tensor memory are released. No barrier tells: a parity wait also succeeds for the phase before the current one, and a
+// stage whose other half was never sent does not complete. What is under way is at most one ring of stages, a few
+// microseconds of work; it gets a millisecond.
+__device__ __forceinline__ void settle() {
+  const unsigned long long t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 1000000ull) {
+  }
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"

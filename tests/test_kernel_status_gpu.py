@@ -1,0 +1,48 @@
+"""The status word of the tensor-core launches: what a call does while it is set, as it is after a bounded wait expired."""
+import pytest
+import torch
+
+from tests.test_linear_cross_entropy_gpu import make
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture
+def word(cuda):
+    """The device's status word; reset and reported afterwards whatever a test did."""
+    from evox_b200.lora_kernels import raise_on_kernel_errors, status_word
+
+    raise_on_kernel_errors()
+    yield status_word(cuda)
+    status_word(cuda).zero_()
+    raise_on_kernel_errors()
+
+
+def population(cuda, pop=4, batch=64, k=256, vocab=700):
+    g = torch.Generator().manual_seed(0)
+    h = torch.randn(pop, batch, k, generator=g).bfloat16().to(cuda)
+    w = (torch.randn(vocab, k, generator=g) / k**0.5).bfloat16().to(cuda)
+    return h, w, torch.arange(pop, device=cuda), 0, 0.05, torch.randint(0, vocab, (batch,), generator=g).to(cuda)
+
+
+@gpu
+@pytest.mark.parametrize("rows,hidden,vocab", [(300, 256, 5000), (20, 512, 3000), (1, 2048, 4096), (2000, 2048, 9000)])
+def test_launches_end_while_the_word_is_set_and_work_when_it_is_not(cuda, word, rows, hidden, vocab):
+    from evox_b200.lora_kernels import lora_layer_cross_entropy
+    from evox_b200.loss_kernels import linear_cross_entropy, linear_cross_entropy_grad
+
+    h, w, labels, b = make(rows, hidden, vocab, torch.bfloat16, True)
+    people = population(cuda)
+
+    def run():
+        return [linear_cross_entropy(h, w, labels, b, reduction="none"), *linear_cross_entropy_grad(h, w, labels, b), lora_layer_cross_entropy(*people)]
+
+    want = run()
+    for code in (1, 3, 4):
+        word.fill_(code)
+        run()
+        torch.cuda.synchronize()
+        assert int(word) == code  # the first report stays
+    word.zero_()
+    for x, y in zip(want, run()):
+        assert torch.equal(x, y)
