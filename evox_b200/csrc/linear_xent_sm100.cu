@@ -403,6 +403,18 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
       }
       if (!ready) {
         settle();
+        // what this warp still had to write becomes NaN: memory that nothing wrote must not pass for a gradient. (Losses and
+        // exponentials need no such care: the status word turns them into NaN when the rows are joined.)
+        for (int left = i; MODE == kOut && left < n_items; ++left) {
+          const Item u = item(left);
+          const Product& q = a.p[u.which];
+          const long long first = (long long)u.m * TM + cta_rank * 128 + quarter * 32, from = (long long)u.n * TN + half * kSlice;
+          for (long long r = first; r < min(first + 32, q.M); ++r)
+            for (long long c = from + lane; c < min(from + kSlice, q.N); c += 32) {
+              if (q.out16) reinterpret_cast<unsigned short*>(q.out16)[r * q.N + c] = 0x7fffu;
+              else q.out32[((long long)u.split * q.M + r) * q.ld32 + c] = NAN;
+            }
+        }
         break;
       }
       if constexpr (MODE == kOut) {
@@ -772,7 +784,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8u * buf);
       }
       if constexpr (MODE == kOut) {
-        if (!ok) break;
+        if (!ok) {  // NaN for what is left, as in xent_product_kernel
+          if (live)
+            for (int j = 0; j < live_tokens; ++j) {
+              if (a.out32) a.out32[((long long)split * a.rows + token0 + j) * a.ld32 + row] = NAN;
+              else a.out16[(long long)(token0 + j) * a.M + row] = 0x7fffu;
+            }
+          continue;
+        }
         const float scale = a.scale ? __ldg(a.scale) : 1.0f;
         if (live) {
 #pragma unroll
@@ -895,11 +914,12 @@ __device__ void row_weights(const Weights& a, long long ignore_index) {
 
 // loss[i] and norm[i] = (maximum, 1 / sum of exponentials) from the slices' pairs: lanes are rows, warps share the slices.
 // The two stay apart: added into one log-sum-exp, the logarithm would vanish next to a maximum of large size. A label outside the
-// vocabulary that is not ignore_index gives NaN (and NaN gradients): loud, and nothing is read out of bounds.
+// vocabulary that is not ignore_index gives NaN (and NaN gradients): loud, and nothing is read out of bounds. Where the status
+// word says that a launch gave up every loss is NaN, and by way of norm every gradient: the slices may never have been written.
 __global__ void __launch_bounds__(1024)
     xent_finish_kernel(const float2* __restrict__ stats, long long ld_stats, int slices, const float* __restrict__ label_logit,
                        const long long* __restrict__ labels, long long label_period, long long ignore_index, long long rows, long long vocab,
-                       float2* __restrict__ norm, float* __restrict__ loss, const Weights weights) {
+                       float2* __restrict__ norm, float* __restrict__ loss, const int* __restrict__ status, const Weights weights) {
   overlapped_start();
   if (weights.scalars && blockIdx.x == gridDim.x - 1) {  // one block more than the rows need
     row_weights(weights, ignore_index);
@@ -908,6 +928,7 @@ __global__ void __launch_bounds__(1024)
   __shared__ float sm[32][33], ss[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long row = (long long)blockIdx.x * 32 + lane;
+  const bool failed = __ldcg(status) != 0;
   float m = -INFINITY, s = 0.f;
   if (row < rows) {
 #pragma unroll 4
@@ -932,8 +953,8 @@ __global__ void __launch_bounds__(1024)
   if (lane == 0) {
     const long long y = labels[mine % label_period];
     const bool ignored = y == ignore_index, outside = !ignored && (y < 0 || y >= vocab);
-    if (norm) norm[mine] = make_float2(m, outside ? NAN : 1.0f / s);
-    loss[mine] = ignored ? 0.f : (outside ? NAN : (m - label_logit[mine]) + logf(s));
+    if (norm) norm[mine] = make_float2(m, outside || failed ? NAN : 1.0f / s);
+    loss[mine] = failed ? NAN : ignored ? 0.f : (outside ? NAN : (m - label_logit[mine]) + logf(s));
   }
 }
 
@@ -944,7 +965,7 @@ constexpr int kJoinWords = 2048;
 __global__ void __launch_bounds__(256)
     xent_logits_kernel(const float* __restrict__ partial, int splits, long long ld, const float* __restrict__ bias,
                        const long long* __restrict__ labels, long long ignore_index, int rows, long long vocab, float2* parts,
-                       float* label_logit, int* tickets, float* __restrict__ loss, const Weights weights) {
+                       float* label_logit, int* tickets, float* __restrict__ loss, const int* __restrict__ status, const Weights weights) {
   overlapped_start();
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (row == rows) {
@@ -953,6 +974,7 @@ __global__ void __launch_bounds__(256)
   }
   __shared__ float sm[8], ss[8];
   __shared__ int last;
+  const bool failed = __ldcg(status) != 0;
   const long long label = labels[row];
   float z[8];
 #pragma unroll
@@ -1013,7 +1035,7 @@ __global__ void __launch_bounds__(256)
   s = warp_sum(s * rescale_to(mine, m));
   if (lane == 0) {
     const bool ignored = label == ignore_index, outside = !ignored && (label < 0 || label >= vocab);
-    loss[row] = ignored ? 0.f : (outside ? NAN : (m - __ldcg(label_logit + row)) + logf(s));
+    loss[row] = failed ? NAN : ignored ? 0.f : (outside ? NAN : (m - __ldcg(label_logit + row)) + logf(s));
   }
 }
 
@@ -1545,10 +1567,11 @@ struct Head {
 };
 
 int finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
-           long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const Weights& weights, cudaStream_t stream) {
+           long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const int* status, const Weights& weights,
+           cudaStream_t stream) {
   const int slices = (int)((vocab + kSlice - 1) / kSlice);
   EVOX_CUDA(launch_overlapped(xent_finish_kernel, dim3((unsigned)((rows + 31) / 32 + (weights.scalars ? 1 : 0))), 1024, 0, 1, stream, stats,
-                              ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, weights));
+                              ld_stats, slices, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, status, weights));
   return EVOX_OK;
 }
 
@@ -1647,7 +1670,7 @@ int few_loss_pass(const Head& x, const Buffers& b, float* loss, const Weights& w
   if (int rc = launch_few<kOut, false, FP16>(map_a, x.h, x.hidden, x.ld_h, a, x.stream)) return rc;
   const dim3 grid((unsigned)((x.vocab + kJoinWords - 1) / kJoinWords), (unsigned)(x.rows + (weights.scalars ? 1 : 0)));
   EVOX_CUDA(launch_overlapped(xent_logits_kernel, grid, 256, 0, 1, x.stream, b.few_logits, a.splits, a.ld32, x.bias, x.labels, x.ignore_index,
-                              a.rows, x.vocab, b.few_parts, b.label_logit, b.few_tickets, loss, weights));
+                              a.rows, x.vocab, b.few_parts, b.label_logit, b.few_tickets, loss, x.error_flag, weights));
   return EVOX_OK;
 }
 
@@ -1686,7 +1709,8 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
     const bool first = r0 == 0, last = r0 + n == x.rows;
     if (int rc = b.e_low ? logits_pass<kProbLow, FP16>(x, b, r0, n, chunk) : logits_pass<kProb, FP16>(x, b, r0, n, chunk)) return rc;
     const Weights weights = {x.labels, x.rows, reduction, grad_loss, kProbScale<FP16>, first ? b.scalars : nullptr};
-    if (int rc = finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, row_loss + r0, weights, x.stream))
+    if (int rc = finish(b.stats, chunk, b.label_logit, x.labels + r0, n, x.ignore_index, n, x.vocab, b.norm, row_loss + r0, x.error_flag, weights,
+                        x.stream))
       return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
     const int column_blocks = (int)((x.vocab + 1023) / 1024), block_rows = rescale_rows(n, x.vocab);
@@ -1761,8 +1785,8 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
 }  // namespace
 
 int xent_finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
-                long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, cudaStream_t stream) {
-  return finish(stats, ld_stats, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, Weights{}, stream);
+                long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const int* status, cudaStream_t stream) {
+  return finish(stats, ld_stats, label_logit, labels, label_period, ignore_index, rows, vocab, norm, loss, status, Weights{}, stream);
 }
 
 }  // namespace evox
@@ -1798,7 +1822,7 @@ extern "C" int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void
     if (int rc = fp16 ? few_loss_pass<true>(x, b, row_loss, weights) : few_loss_pass<false>(x, b, row_loss, weights)) return rc;
   } else {
     if (int rc = fp16 ? logits_pass<kLoss, true>(x, b, 0, rows, rows) : logits_pass<kLoss, false>(x, b, 0, rows, rows)) return rc;
-    if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, row_loss, weights, s)) return rc;
+    if (int rc = finish(b.stats, rows, b.label_logit, x.labels, rows, ignore_index, rows, vocab, nullptr, row_loss, x.error_flag, weights, s)) return rc;
   }
   if (!per_row) {
     EVOX_CUDA(launch_overlapped(xent_loss_sum_kernel, dim3(1), 256, 0, 1, s, b.loss, rows, b.scalars, loss));

@@ -1032,7 +1032,7 @@ extern "C" int evox_lora_cross_entropy_bf16(const void* h, const void* w, const 
   a.stats = reinterpret_cast<float2*>(workspace);
   a.label_logit = reinterpret_cast<float*>(a.stats + a.M * ((vocab + kSlice - 1) / kSlice));
   if (int rc = launch_gemm(h, a.M, w, vocab, k, a, false, s)) return rc;
-  return xent_finish(a.stats, a.M, a.label_logit, a.labels, batch, ignore_index, a.M, vocab, nullptr, loss, s);
+  return xent_finish(a.stats, a.M, a.label_logit, a.labels, batch, ignore_index, a.M, vocab, nullptr, loss, error_flag, s);
 }
 
 extern "C" int evox_neg_mse_from_partials(const float* row_partial, int64_t pop, int64_t batch, int64_t d, float* fitness,

@@ -50,8 +50,8 @@ __device__ __forceinline__ void keep_label(const float (&z)[32], long long label
 }
 
 // loss[i] (and norm[i] = (maximum, 1 / sum), if not null) of `rows` rows from stats[slice][row] and the labels' logits; row i
-// has label labels[i % label_period].
+// has label labels[i % label_period]. NaN if the status word is set.
 int xent_finish(const float2* stats, long long ld_stats, const float* label_logit, const long long* labels, long long label_period,
-                long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, cudaStream_t stream);
+                long long ignore_index, long long rows, long long vocab, float2* norm, float* loss, const int* status, cudaStream_t stream);
 
 }  // namespace evox

@@ -27,8 +27,9 @@ _pending_flags: list[tuple[str, torch.Tensor]] = []
 
 
 def raise_on_kernel_errors() -> None:
-    """Synchronise on and check every tensor-core launch since the last call; raise if a bounded
-    device-side wait expired (1 producer, 2 / 3 issuer, 4 epilogue) or shared memory was misaligned (5)."""
+    """Check the tensor-core launches since the last call that the current stream comes after (its own, and those of streams
+    it waited for): waits for them, and raises if a bounded device-side wait expired (1 producer, 2 / 3 issuer, 4 epilogue)
+    or shared memory was misaligned (5). During a capture nothing can be read and nothing is checked."""
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         return  # nothing can be read back now
     for index, word in _status_words.items():
@@ -43,8 +44,8 @@ def raise_on_kernel_errors() -> None:
             raise _cabi.EvoxKernelError(f"{what}: the tensor-core kernel gave up with status {code} (a bounded wait expired)")
 
 
-# One status word per device for the launches that share theirs: a kernel writes it only when a wait expires, and the
-# launches after that give up as well until `raise_on_kernel_errors` has reported it.
+# One status word per device for the cross-entropy launches: a kernel writes it only when a wait expires. From then on
+# their results are NaN, those of that launch first, until `raise_on_kernel_errors` has reported it.
 _status_words: dict[int, torch.Tensor] = {}
 
 
@@ -222,7 +223,8 @@ def lora_layer_cross_entropy(h: torch.Tensor, w: torch.Tensor, seeds: torch.Tens
     """Cross entropy of a virtual-LoRA vocabulary head on the tensor cores: the losses (pop, batch), fp32, of
     `lora_layer_bf16`'s layer (same arguments; w (vocab, k) of any vocab) against class `labels` (batch,) shared by the population.
     The epilogue reduces the logits to softmax statistics, so (pop, batch, vocab) never exists. A token labelled `ignore_index`
-    has loss 0, another label outside the vocabulary gives NaN."""
+    has loss 0, another label outside the vocabulary gives NaN. So does a launch that gave up (`raise_on_kernel_errors` says
+    so and clears the device's status word)."""
     rank = 8
     err = _cabi.EvoxKernelError
     if h.ndim != 3 or w.ndim != 2 or h.shape[2] != w.shape[1]:

@@ -4,6 +4,10 @@
 epilogue reduces every row to its log-sum-exp, so the (rows, vocab) logits never exist. It is differentiable;
 `linear_cross_entropy_grad` returns loss and gradients in one call, without autograd. The same loss for a
 virtual-LoRA population is `lora_kernels.lora_layer_cross_entropy`.
+
+Every device-side wait is bounded. If one expires, that call and those after it on the device give NaN, losses and
+gradients alike, until `lora_kernels.raise_on_kernel_errors` has raised it (a wait for the current stream; once per epoch or
+wherever a loss is looked at is enough).
 """
 
 from __future__ import annotations

@@ -583,7 +583,8 @@ int evox_bench_compare_rate(const float* in, uint32_t* out, int32_t iterations, 
  * loss 0; any other label outside [0, vocab) gives NaN. loss: rows values (EVOX_REDUCE_NONE) or one.
  * The logits are not stored: the workspace holds 8 bytes per row and 128 columns. error_flag: a
  * device int32 that holds 0, set to a status if a bounded device-side wait expired; one word may serve
- * any number of calls. */
+ * any number of calls. While it is set, by this call or an earlier one, losses and gradients come out as
+ * NaN. */
 int32_t evox_linear_cross_entropy_copies(const void* h, int64_t ld_h, const void* w, int64_t ld_w);
 size_t evox_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab,
                                                  int32_t copies);
