@@ -159,21 +159,36 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+inline int driver_entry(const char* name, void** out) {
+  cudaDriverEntryPointQueryResult q;
+  EVOX_CUDA(cudaGetDriverEntryPoint(name, out, cudaEnableDefault, &q));
+  EVOX_REQUIRE(*out != nullptr && q == cudaDriverEntryPointSuccess, EVOX_ERR_CUDA, "%s is not available", name);
+  return EVOX_OK;
+}
+
 inline int encode_fn(EncodeTiledFn* out) {
+  typedef CUresult (*CurrentFn)(CUcontext*);
   static EncodeTiledFn fn = nullptr;
+  static CurrentFn current = nullptr;
   static std::mutex mu;
   std::lock_guard<std::mutex> lock(mu);
   if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    EVOX_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-    EVOX_REQUIRE(p != nullptr && q == cudaDriverEntryPointSuccess, EVOX_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    fn = reinterpret_cast<EncodeTiledFn>(p);
+    void *encode = nullptr, *get = nullptr;
+    if (int rc = driver_entry("cuTensorMapEncodeTiled", &encode)) return rc;
+    if (int rc = driver_entry("cuCtxGetCurrent", &get)) return rc;
+    current = reinterpret_cast<CurrentFn>(get);
+    fn = reinterpret_cast<EncodeTiledFn>(encode);
   }
-  // the encoder is a driver call: a thread that made no runtime call yet (one of autograd's) has no context to make it in
+  // the encoder is a driver call: a thread that made no runtime call yet (one of autograd's) has no context to make it in.
+  // Setting the device that is current anyway makes one, and is allowed while a stream is being captured.
   static thread_local bool bound = false;
   if (!bound) {
-    EVOX_CUDA(cudaFree(nullptr));
+    CUcontext context = nullptr;
+    if (current(&context) != CUDA_SUCCESS || context == nullptr) {
+      int dev = 0;
+      EVOX_CUDA(cudaGetDevice(&dev));
+      EVOX_CUDA(cudaSetDevice(dev));
+    }
     bound = true;
   }
   *out = fn;
