@@ -712,6 +712,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int work = first; work < n_work && ok; work += step) {
         const int split = work / a.tiles, begin = split_begin(split), count = split_begin(split + 1) - begin;
+        // floor(chunk count / chunks); with up to 2^16 chunks (2^26 features) no product here leaves 32 bits
+        const unsigned each = (unsigned)count / (unsigned)chunks, more = (unsigned)count - each * (unsigned)chunks;
+        auto chunk_begin = [&](unsigned chunk) { return (int)(chunk * each + chunk * more / (unsigned)chunks); };
         for (int chunk = 0; chunk < chunks && ok; ++chunk, ++it) {
           const int buf = it & 1;
           if (!mbar_wait(tempty_bar(buf), (uint32_t)((it >> 1) & 1) ^ 1u, a.error_flag, 2)) {
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_after_sync();
           const uint32_t d_tmem = tmem_base + (uint32_t)(buf * kFewSums * NT);
-          const int kb0 = chunk * count / chunks, kb1 = (chunk + 1) * count / chunks;
+          const int kb0 = chunk_begin(chunk), kb1 = chunk_begin(chunk + 1);
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait(full_bar(s), ph, a.error_flag, 3)) {
               ok = false;
