@@ -1058,6 +1058,7 @@ __device__ void sum_losses(const float* __restrict__ loss, long long rows, const
   }
 }
 
+constexpr int kRescaleColumns = 1024;  // columns of a block of the rescaling pass
 // e -> g in place (see the head of the file), `block_rows` (at most 32) rows x 1,024 columns per block, eight columns per
 // thread; column sums of the block's rows for the bias gradient, which is a 32-bit result: they take e with what its
 // rounding left. The blocks of one more grid row copy the hidden states for the weight gradient, with zeros where the
@@ -1108,7 +1109,7 @@ __global__ void __launch_bounds__(256, BIAS ? 3 : 5)
   __shared__ float sums[128][8];
   // backwards: the columns that the product wrote last are still in the L2 cache, and those written here last are the first
   // that the next product reads
-  const long long col_base = (long long)(column_blocks - 1 - (int)blockIdx.y) * 1024;
+  const long long col_base = (long long)(column_blocks - 1 - (int)blockIdx.y) * kRescaleColumns;
   const int group = tid & 127, part = tid >> 7;  // eight columns; even or odd rows
   const long long col = col_base + group * 8;
   unsigned short* column = e + row0 * ld_e + col;
@@ -1716,7 +1717,7 @@ int gradient_pass(const Head& x, const Buffers& b, long long chunk, int reductio
                         x.stream))
       return rc;
     const unsigned short* h = reinterpret_cast<const unsigned short*>(x.h) + r0 * x.ld_h;
-    const int column_blocks = (int)((x.vocab + 1023) / 1024), block_rows = rescale_rows(n, x.vocab);
+    const int column_blocks = (int)((x.vocab + kRescaleColumns - 1) / kRescaleColumns), block_rows = rescale_rows(n, x.vocab);
     const int row_blocks = (int)((n + block_rows - 1) / block_rows);
     const bool sum_here = last && !per_row;
     EVOX_CUDA(launch_overlapped(
@@ -1855,6 +1856,9 @@ extern "C" int evox_linear_cross_entropy_grad(const void* h, int64_t ld_h, const
   if (int rc = check_operands("linear_cross_entropy_grad", h, ld_h, w, ld_w, dtype, labels, rows, hidden, vocab, reduction, loss, workspace, error_flag))
     return rc;
   EVOX_REQUIRE(chunk_rows > 0, EVOX_ERR_INVALID, "linear_cross_entropy_grad: chunk_rows must be positive");
+  // the rescaling pass has a grid row per kRescaleColumns columns and two more; a grid has 65,535
+  EVOX_REQUIRE(vocab <= 65533ll * kRescaleColumns, EVOX_ERR_INVALID, "linear_cross_entropy_grad: vocab must be at most %lld, got %lld",
+               65533ll * kRescaleColumns, (long long)vocab);
   const long long chunk = chunk_rows < rows ? chunk_rows : rows;
   Buffers b = {};
   EVOX_REQUIRE(workspace_bytes >= layout(b, workspace, rows, hidden, vocab, copies_of(h, ld_h, w, ld_w), chunk, true, dbias != nullptr), EVOX_ERR_WORKSPACE,

@@ -125,7 +125,7 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
     """Loss and its gradients in one call: `(loss, dh, dweight, dbias)`, the gradients in their operands' types
     (`dbias` is None without a bias). Arguments as for `linear_cross_entropy`; `grad_loss` is the upstream gradient
     (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
-    are held at a time (default: all, up to 2 GiB of them)."""
+    are held at a time (default: all, up to 2 GiB of them; a bias gradient doubles the bytes)."""
     _check_chunk(chunk_rows)
     flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
     if grad_loss is not None:
@@ -183,7 +183,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     have loss 0, do not count in the mean and get zero gradients, whatever they hold; a label
     outside the vocabulary gives NaN. `reduction`: "mean", "sum" or "none" (losses shaped like `labels`).
     Differentiable once in `h`, `weight` and `bias`; the gradient holds 16-bit exponentials of `chunk_rows` rows at a time
-    (default: all, up to 2 GiB of them)."""
+    (default: all, up to 2 GiB of them; a bias gradient doubles the bytes)."""
     _check_chunk(chunk_rows)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _LinearCrossEntropy.apply(h, weight, labels, bias, ignore_index, reduction, chunk_rows)

@@ -598,7 +598,8 @@ int evox_linear_cross_entropy(const void* h, int64_t ld_h, const void* w, int64_
  * dbias (vocab, fp32); each may be NULL. grad_loss (device, or NULL for 1): the upstream gradient, one
  * value, or one per row with EVOX_REDUCE_NONE. Rows are taken chunk_rows at a time, with 16 bits per
  * logit of one chunk in the workspace; evox_linear_cross_entropy_chunk_rows gives the number that the
- * Python wrapper uses (at most 2 GiB of them). with_bias: whether dbias will be given. */
+ * Python wrapper uses (at most 2 GiB of them; a bias gradient needs as many bytes again, for what the 16 bits
+ * leave). with_bias: whether dbias will be given. vocab is at most 67,105,792 here. */
 int64_t evox_linear_cross_entropy_chunk_rows(int64_t rows, int64_t vocab);
 size_t evox_linear_cross_entropy_grad_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab,
                                                       int64_t chunk_rows, int32_t with_bias,

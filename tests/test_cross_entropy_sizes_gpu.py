@@ -47,3 +47,15 @@ def test_more_features_than_a_32_bit_product_of_blocks_and_chunks(cuda, rows, bi
         near(dw[:, at : at + 2**20], a, moved.t() @ hp.abs() + (u + 2.0**-19) * a.abs() + 2.0**-19 * (size.t() @ hp.abs()) + 1e-30, "dw")
     if bias:
         near(db, grad.sum(dim=0), moved.sum(dim=0), "db")
+
+
+def test_the_largest_vocabulary_of_a_gradient():
+    """One word more than the rescaling pass has blocks for is refused before anything is launched (the addresses are made up)."""
+    from evox_b200 import _cabi
+
+    lib = _cabi.lib
+    good = dict(h=256, ld_h=8, w=256, ld_w=8, dtype=0, bias=None, labels=256, ignore=-100, rows=4, hidden=8, vocab=67_105_793, reduction=0, grad_loss=None,
+                chunk=4, loss=256, dh=256, dw=256, db=None, ws=256, nbytes=0, err=256, stream=None)
+    assert lib.evox_linear_cross_entropy_grad(*good.values()) == -1
+    assert b"vocab must be at most 67105792" in lib.evox_last_error()
+    assert lib.evox_linear_cross_entropy_grad(*{**good, "vocab": 67_105_792}.values()) == -3  # this one has no workspace
