@@ -13,6 +13,7 @@ wherever a loss is looked at is enough).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 from .lora_kernels import status_word
@@ -72,6 +73,12 @@ def _arguments(h, weight, labels, bias, reduction):
     return h, weight, labels, bias, rest
 
 
+def _refuse_tangents(*tensors) -> None:
+    """Forward-mode tangents would be dropped without a word: the kernels see values only."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _cabi.EvoxKernelError("linear_cross_entropy has no forward-mode derivative: an argument carries a tangent")
+
+
 def _check_chunk(chunk_rows: int | None) -> None:
     if chunk_rows is not None and chunk_rows < 1:
         raise _cabi.EvoxKernelError(f"chunk_rows must be at least 1, got {chunk_rows}")
@@ -127,6 +134,7 @@ def linear_cross_entropy_grad(h: torch.Tensor, weight: torch.Tensor, labels: tor
     (one fp32 value, or one per row with `reduction="none"`). `chunk_rows`: rows whose 16-bit exponentials
     are held at a time (default: all, up to 2 GiB of them; a bias gradient doubles the bytes)."""
     _check_chunk(chunk_rows)
+    _refuse_tangents(h, weight, bias, grad_loss)
     flat, weight, labels, bias_f, shape = _arguments(h, weight, labels, bias, reduction)
     if grad_loss is not None:
         want = shape if reduction == "none" else ()
@@ -182,9 +190,10 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     start on 16-byte boundaries are copied); `labels` (...) int64; `bias` (vocab,). Rows labelled `ignore_index`
     have loss 0, do not count in the mean and get zero gradients, whatever they hold; a label
     outside the vocabulary gives NaN. `reduction`: "mean", "sum" or "none" (losses shaped like `labels`).
-    Differentiable once in `h`, `weight` and `bias`; the gradient holds 16-bit exponentials of `chunk_rows` rows at a time
+    Differentiable once in `h`, `weight` and `bias`, in reverse mode (a forward-mode tangent is refused); the gradient holds 16-bit exponentials of `chunk_rows` rows at a time
     (default: all, up to 2 GiB of them; a bias gradient doubles the bytes)."""
     _check_chunk(chunk_rows)
+    _refuse_tangents(h, weight, bias)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _LinearCrossEntropy.apply(h, weight, labels, bias, ignore_index, reduction, chunk_rows)
     return _loss(*_arguments(h, weight, labels, bias, reduction)[:4], ignore_index, reduction, tuple(h.shape[:-1]))

@@ -111,3 +111,35 @@ def test_backward_under_a_loss_scale_in_a_graph(cuda, dtype):
                 assert torch.equal(x * factor, y)
             else:  # below 2^-14 the scaled gradient has fewer digits
                 assert bool(((x.double() * factor - y.double()).abs() <= 2.0**-11 * (x.double() * factor).abs() + 2.0**-24).all())
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require grad; without a look at its tangent the loss would come out as a constant."""
+    import torch.autograd.forward_ad as fw
+
+    from evox_b200._cabi import EvoxKernelError
+    from evox_b200.loss_kernels import linear_cross_entropy, linear_cross_entropy_grad
+
+    h, w, y, b = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(9, 16, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64), torch.zeros(9)
+    with fw.dual_level():
+        for i in (0, 1, 3):
+            args = [h, w, y, b]
+            args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+            for fn in (linear_cross_entropy, linear_cross_entropy_grad):
+                with pytest.raises(EvoxKernelError, match="forward-mode"):
+                    fn(*args)
+        for fn in (linear_cross_entropy, linear_cross_entropy_grad):  # no tangent: refused for being on the host only
+            with pytest.raises(EvoxKernelError, match="CUDA device"):
+                fn(h, w, y, b)
+
+
+@gpu
+def test_values_without_a_tangent_pass_inside_a_dual_level(cuda):
+    import torch.autograd.forward_ad as fw
+
+    from evox_b200.loss_kernels import linear_cross_entropy
+
+    h, w, labels, b = make(40, 64, 300, torch.bfloat16, True)
+    want = linear_cross_entropy(h, w, labels, b)
+    with fw.dual_level():
+        assert torch.equal(linear_cross_entropy(h, w, labels, b), want)
