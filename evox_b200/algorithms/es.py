@@ -65,7 +65,8 @@ class _ESBase(Algorithm):
     def _set_max_grad_norm(self, max_grad_norm: float | None) -> None:
         assert max_grad_norm is None or max_grad_norm > 0, "max_grad_norm must be greater than 0."
         self.max_grad_norm = max_grad_norm
-        self.grad_norm = None  # 0-d tensor: the norm before clipping, of the latest step
+        # state like any other, so that traced and mapped steps keep it too: the norm before clipping, of the latest step
+        self.grad_norm = None if max_grad_norm is None else Mutable(torch.full((), float("nan"), device=self.center.device))
 
     def _clip(self, grads: list[torch.Tensor]) -> None:
         """Scale the gradient (all its blocks) to at most `max_grad_norm`, in place."""
@@ -74,7 +75,7 @@ class _ESBase(Algorithm):
         if torch.compiler.is_compiling():
             from .. import ops
 
-            ops.clip_grad_norm_(grads, self.max_grad_norm)
+            self.grad_norm = ops.clip_grad_norm_(grads, self.max_grad_norm)
         else:
             self.grad_norm = clip_grad_norm_(grads, self.max_grad_norm)
 
@@ -109,7 +110,8 @@ class OpenES(_ESBase):
         device: torch.device | None = None,
         max_grad_norm: float | None = None,
     ):
-        """`max_grad_norm`: the gradient is scaled down to this 2-norm before the update (`grad_norm` keeps the norm it had)."""
+        """`max_grad_norm`: the gradient is scaled down to this 2-norm before the update (`grad_norm`, 0-d, keeps the norm it
+        had; NaN before the first step)."""
         super().__init__()
         device = torch.get_default_device() if device is None else torch.device(device)
         if mirrored_sampling is True:
@@ -399,7 +401,7 @@ class VirtualLoRAES(_ESBase):
         centre, but the gradient and update of each 2-D block are computed for this rank's rows only
         and the updated rows are allgathered; seeds are broadcast from rank 0 each generation.
         `max_grad_norm`: the gradient over all blocks is scaled down to this 2-norm before the update (`grad_norm`
-        keeps the norm it had); all blocks are then held at once. Not with `shard=True`: no rank has the whole gradient."""
+        keeps the norm it had, NaN before the first step); all blocks are then held at once. Not with `shard=True`: no rank has the whole gradient."""
         super().__init__()
         device = torch.get_default_device() if device is None else torch.device(device)
         self.group = group
