@@ -451,13 +451,18 @@ class VirtualLoRAES(_ESBase):
             start += n
 
     def _clipped_update(self, fitness: torch.Tensor, sigma: float) -> None:
-        """The whole gradient, a block after the other in the centre's order, clipped, then one update."""
-        grad = torch.empty_like(self.center)
-        blocks = list(grad.split([int(torch.tensor(s).prod()) for s in self.param_shapes]))
-        for shape, offset, block in zip(self.param_shapes, self.counter_offsets, blocks):
-            lora_gradient_from_seeds(fitness, self.seeds, shape, self.lora_rank, offset, self.pop_size, sigma, out=block, passes=self.gradient_passes)
-        self._clip(blocks)
-        _update_center(self, grad)
+        """The whole gradient, clipped, then the update. Every block has a buffer of its own, as without a bound: a piece of one
+        buffer that starts off 16 bytes (after a block of odd length) would leave the tensor cores for another kernel and
+        its rounding."""
+        sizes = [int(torch.tensor(s).prod()) for s in self.param_shapes]
+        grads = [torch.empty(n, dtype=torch.float32, device=self.center.device) for n in sizes]
+        for shape, offset, grad in zip(self.param_shapes, self.counter_offsets, grads):
+            lora_gradient_from_seeds(fitness, self.seeds, shape, self.lora_rank, offset, self.pop_size, sigma, out=grad, passes=self.gradient_passes)
+        self._clip(grads)
+        start = 0
+        for n, grad in zip(sizes, grads):
+            _update_center(self, grad, start, n)
+            start += n
 
     def _row_shard(self, shape) -> tuple[int, int] | None:
         """This rank's rows of a 2-D block, or None when the block is not sharded (1-D blocks, a
