@@ -17,8 +17,6 @@ __all__ = [
     "lora_delta_output", "lora_gradient", "lora_gradient_from_seeds", "lora_layer_bf16", "lora_layer_cross_entropy", "raise_on_kernel_errors",
 ]
 
-_grad_ws: dict[torch.device, torch.Tensor] = {}
-
 # Error flags of tensor-core launches that have not been looked at yet. The kernels bound every wait
 # and report an expired one through a device word; reading it needs a host synchronisation, so the
 # flags are collected here and examined by `raise_on_kernel_errors()` (the problem / algorithm
@@ -293,14 +291,12 @@ def lora_gradient_from_seeds(fitness: torch.Tensor, seeds: torch.Tensor, weight_
         if _cabi.lib.evox_lora_gradient_tc_supported(pop_size, r1 - r0, k, rank) and out.data_ptr() % 16 == 0:
             d = r1 - r0
             nbytes = _cabi.lib.evox_lora_gradient_tc_workspace_bytes(pop_size, d, k)
-            ws = _grad_ws.get(dev)
-            if ws is None or ws.numel() < nbytes:
-                ws = _grad_ws[dev] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call: others may run on other streams, or in graphs
             err = torch.zeros(1, dtype=torch.int32, device=dev)
             _cabi.check(
                 _cabi.lib.evox_lora_gradient_tc(
                     _cabi.ptr(fitness), _cabi.ptr(seeds), counter, pop_size, float(sigma), r0, d, k, rank, passes, _cabi.ptr(out),
-                    _cabi.ptr(ws), ws.numel(), _cabi.ptr(err), _cabi.stream_ptr(dev),
+                    _cabi.ptr(ws), nbytes, _cabi.ptr(err), _cabi.stream_ptr(dev),
                 )
             )
             lora_gradient_from_seeds.last_error_flag = err

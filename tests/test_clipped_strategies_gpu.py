@@ -91,3 +91,88 @@ def test_without_a_bound_there_is_no_norm():
     assert algo.grad_norm is None and "grad_norm" not in algo.state_dict()
     algo = OpenES(4, torch.zeros(3), 0.1, 0.1, device="cpu", max_grad_norm=1.0)
     assert torch.isnan(algo.grad_norm) and algo.grad_norm.shape == () and "grad_norm" in algo.state_dict()
+
+
+class Recorder:
+    """The library, with the workspace addresses of the gradient's calls written down."""
+
+    def __init__(self, lib):
+        self._lib, self.workspaces = lib, []
+
+    def __getattr__(self, name):
+        fn = getattr(self._lib, name)
+        if name != "evox_lora_gradient_tc":
+            return fn
+        return lambda *a: (self.workspaces.append(a[11]), fn(*a))[1]
+
+
+@gpu
+def test_gradients_under_way_at_once_share_no_workspace(cuda, monkeypatch):
+    """Two streams, and a captured call next to eager ones: the operand pieces of one must not land on another's."""
+    from evox_b200 import _cabi
+    from evox_b200.lora_kernels import lora_gradient_from_seeds
+
+    g = torch.Generator().manual_seed(0)
+    fitness = [torch.randn(64, generator=g).to(cuda) for _ in range(3)]
+    seeds = [torch.arange(64).to(cuda) + 1000 * i for i in range(3)]
+
+    def gradient(i):
+        return lora_gradient_from_seeds(fitness[i], seeds[i], (512, 1024), 8, 40, 64, 0.1)
+
+    want = [gradient(i) for i in range(3)]
+    torch.cuda.synchronize()
+    recorder = Recorder(_cabi.lib)
+    monkeypatch.setattr(_cabi, "lib", recorder)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(gradient(i))
+        torch.cuda.synchronize()
+        for x, y in zip(want, got):
+            assert torch.equal(x, y)
+    first, second = set(recorder.workspaces[0::2]), set(recorder.workspaces[1::2])
+    assert not first & second
+    graph = torch.cuda.CUDAGraph()
+    recorder.workspaces.clear()
+    with torch.cuda.graph(graph):
+        captured = gradient(2)
+    with torch.cuda.stream(streams[0]):
+        eager = gradient(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert recorder.workspaces[0] != recorder.workspaces[1]
+    assert torch.equal(captured, want[2]) and torch.equal(eager, want[0])
+
+
+@gpu
+def test_clipped_updates_on_two_streams(cuda):
+    from evox_b200.algorithms import VirtualLoRAES
+
+    shapes = [(256, 512), (5,), (512, 256)]
+    dim = sum(int(torch.tensor(s).prod()) for s in shapes)
+    g = torch.Generator().manual_seed(0)
+    centers = [torch.randn(dim, generator=g).to(cuda) for _ in range(2)]
+    fits = [torch.randn(32, generator=g).to(cuda) for _ in range(2)]
+    seeds = [(torch.arange(32) + 100 * i).to(cuda) for i in range(2)]
+
+    def strategy(i):
+        algo = VirtualLoRAES(shapes, 8, 32, centers[i], 0.1, 0.05, device=cuda, max_grad_norm=0.5)
+        algo.evaluate = lambda payload: fits[i]
+        return algo
+
+    serial = [strategy(i) for i in range(2)]
+    for i, algo in enumerate(serial):
+        for _ in range(3):
+            algo.step(seeds[i])
+    torch.cuda.synchronize()
+    streams, both = [torch.cuda.Stream() for _ in range(2)], [strategy(i) for i in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i, algo in enumerate(both):
+            with torch.cuda.stream(streams[i]):
+                algo.step(seeds[i])
+    torch.cuda.synchronize()
+    for x, y in zip(serial, both):
+        assert torch.equal(x.center, y.center) and torch.equal(x.grad_norm, y.grad_norm)
