@@ -18,13 +18,33 @@ from torch import nn
 from .. import _cabi
 from ..core import Problem
 from ..lora_kernels import (
-    compute_counter_offsets, generate_lora_factors, lora_layer_bf16, lora_layer_cross_entropy, raise_on_kernel_errors,
+    compute_counter_offsets, generate_lora_factors, lora_layer_bf16, lora_layer_cross_entropy, philox_normal, raise_on_kernel_errors,
 )
 from ..sharding import group_info, shard_bounds
 
 __all__ = ["VirtualLoRAProblem"]
 
 _ACTIVATIONS = (nn.ReLU, nn.Tanh, nn.Sigmoid, nn.GELU, nn.LeakyReLU, nn.ELU, nn.Softmax, nn.Identity)
+
+
+def _bf16_pieces(x: torch.Tensor) -> list[torch.Tensor]:
+    """bf16 tensors that add up to `x` (to 2^-26 of each value): `x` itself, or three of falling size."""
+    if x.dtype == torch.bfloat16:
+        return [x]
+    pieces, rest = [], x.to(torch.float32)
+    for _ in range(3):
+        pieces.append(rest.to(torch.bfloat16))
+        rest = rest - pieces[-1]
+    return pieces
+
+
+def _in_bf16_pieces(h: torch.Tensor, w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 operands (pop, batch, n k) and (vocab, n k) whose product is h w^T to fp32's digits: along the reduction every
+    pair of pieces down to 2^-24 of the largest, small ones first so that the accumulator, which truncates when it adds, is
+    small while they come. n is 3 for bf16 activations, 6 for fp32 ones."""
+    hs, ws = _bf16_pieces(h), _bf16_pieces(w)
+    pairs = sorted(((i, j) for i in range(len(hs)) for j in range(len(ws)) if i + j <= 2), key=lambda p: -sum(p))
+    return torch.cat([hs[i] for i, _ in pairs], dim=-1), torch.cat([ws[j] for _, j in pairs], dim=-1)
 
 
 class VirtualLoRAProblem(Problem):
@@ -34,9 +54,10 @@ class VirtualLoRAProblem(Problem):
         """`compute_dtype=torch.bfloat16` runs every Linear layer whose shape the tensor-core kernel
         supports (rank 8, batch 64 or 128 per individual, feature sizes multiples of 256) with bf16
         operands and fp32 accumulation; other layers and the default use the fp32 kernels. A last Linear layer on
-        that path ends in the loss itself, without storing its outputs, for `nn.MSELoss(reduction="none")` and, as
-        a vocabulary head of any number of classes, for `nn.CrossEntropyLoss(reduction="none")` without class
-        weights or label smoothing."""
+        that path ends in the loss itself, without storing its outputs, for `nn.MSELoss(reduction="none")` and
+        `nn.CrossEntropyLoss(reduction="none")` without class weights or label smoothing. With the latter so does a
+        head of any other number of classes (input width a multiple of 128), whose fp32 operands then reach the
+        tensor cores in bf16 pieces that keep their digits."""
         super().__init__()
         self.compute_dtype = compute_dtype
         # shard=True: this rank evaluates only its tensor_split share of the individuals and the
@@ -75,6 +96,15 @@ class VirtualLoRAProblem(Problem):
         n = int(torch.tensor(self.param_shapes[i]).prod())
         return center[self._starts[i] : self._starts[i] + n].view(self.param_shapes[i]), i
 
+    def _project(self, h: torch.Tensor, seeds: torch.Tensor, i: int) -> torch.Tensor:
+        """h A^T (pop, batch, rank) of weight block `i` in fp32."""
+        pop, batch, k = h.shape
+        a = philox_normal(seeds, self.lora_rank * k, self.counter_offsets[i]).view(pop, self.lora_rank, k)
+        t = torch.empty(pop, batch, self.lora_rank, dtype=torch.float32, device=h.device)
+        _cabi.check(_cabi.lib.evox_lora_down(_cabi.ptr(h.to(torch.float32)), 0, _cabi.ptr(a), pop, batch, k, self.lora_rank, _cabi.ptr(t),
+                                             _cabi.stream_ptr(h.device)))
+        return t
+
     def _virtual_forward(self, inputs: torch.Tensor, center: torch.Tensor, seeds: torch.Tensor, sigma: float, pop_size: int,
                          mse_target: torch.Tensor | None = None, class_labels: torch.Tensor | None = None, ignore_index: int = -100):
         """Activations of the last layer, (pop, batch, out) fp32. With `mse_target` (batch, out) and a
@@ -105,9 +135,14 @@ class VirtualLoRAProblem(Problem):
                     if module.bias is not None:
                         bias, bi = self._param(center, f"{name}.bias")
                         bias_counter = self.counter_offsets[bi]
+                    if lib.evox_lora_gemm_supported(pop_size, batch, k, d, self.lora_rank):
+                        operands, t = (h.to(torch.bfloat16), weight.to(torch.bfloat16)), pending_t
+                    else:
+                        operands, t = _in_bf16_pieces(h, weight), self._project(h, seeds, wi)
+                    # with t given the kernel draws B alone, from `counter` + 8 row lengths on: those of the pieces' rows here
+                    counter = self.counter_offsets[wi] + self.lora_rank * (k - operands[1].shape[1])
                     return "cross_entropy", lora_layer_cross_entropy(
-                        h.to(torch.bfloat16), weight.to(torch.bfloat16), seeds, self.counter_offsets[wi], sigma, class_labels, bias=bias,
-                        bias_counter=bias_counter, t=pending_t, ignore_index=ignore_index)
+                        *operands, seeds, counter, sigma, class_labels, bias=bias, bias_counter=bias_counter, t=t, ignore_index=ignore_index)
                 if (self.compute_dtype == torch.bfloat16 and not shared
                         and lib.evox_lora_gemm_supported(pop_size, batch, k, d, self.lora_rank)):
                     bias = bias_counter = None
@@ -125,9 +160,7 @@ class VirtualLoRAProblem(Problem):
                     next_counter = None
                     if not last and isinstance(children[nxt][1], nn.Linear):
                         nd, nk = children[nxt][1].weight.shape
-                        head = class_labels is not None and nxt + 1 == len(children)
-                        if nk == d and (lib.evox_lora_gemm_supported(pop_size, batch, nk, nd, self.lora_rank)
-                                        or (head and lib.evox_lora_cross_entropy_supported(pop_size, batch, nk, nd, self.lora_rank))):
+                        if nk == d and lib.evox_lora_gemm_supported(pop_size, batch, nk, nd, self.lora_rank):
                             next_counter = self.counter_offsets[self.param_names.index(f"{children[nxt][0]}.weight")]
                     res = lora_layer_bf16(
                         h.to(torch.bfloat16), weight.to(torch.bfloat16), seeds, self.counter_offsets[wi], sigma, bias=bias,
