@@ -169,8 +169,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         ignore_index, reduction, shape, h_shape, bias_dtype, chunk_rows = ctx.args
-        if len(ctx.saved_tensors) == 4:
-            h, weight, labels, bias = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        if len(saved) == 4:  # the operands; otherwise gradients
+            h, weight, labels, bias = saved
             flat, w, flat_labels, bias_f, _ = _arguments(h, weight, labels, bias, reduction)
             wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
             with torch.cuda.device(h.device):
@@ -178,7 +179,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                                                grad.to(torch.float32).contiguous(), chunk_rows, wanted)
         else:
             # one element, not a 0-d tensor: that would be rounded to bf16 before the product
-            dh, dw, db = (None if g is None else torch.mul(g, grad.reshape(1), out=torch.empty_like(g)) for g in ctx.saved_tensors)
+            dh, dw, db = (None if g is None else torch.mul(g, grad.reshape(1), out=torch.empty_like(g)) for g in saved)
         return (None if dh is None else dh.view(h_shape), dw, None, None if db is None else db.to(bias_dtype), None, None, None)
 
 

@@ -143,3 +143,28 @@ def test_values_without_a_tangent_pass_inside_a_dual_level(cuda):
     want = linear_cross_entropy(h, w, labels, b)
     with fw.dual_level():
         assert torch.equal(linear_cross_entropy(h, w, labels, b), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,reduction", [(torch.bfloat16, "mean"), (torch.bfloat16, "none"), (torch.float16, "sum")])
+def test_saved_tensors_are_unpacked_once(cuda, dtype, reduction):
+    """Hooks that keep what a graph saves elsewhere (offloading) bring it back once."""
+    from evox_b200.loss_kernels import linear_cross_entropy
+
+    h, w, labels, b = make(40, 64, 300, dtype, True)
+    hs = h.clone().requires_grad_()
+    count = {"pack": 0, "unpack": 0}
+
+    def pack(t):
+        count["pack"] += 1
+        return t.cpu()
+
+    def unpack(t):
+        count["unpack"] += 1
+        return t.cuda()
+
+    want, = torch.autograd.grad(linear_cross_entropy(hs, w, labels, b, reduction=reduction).sum(), hs)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        loss = linear_cross_entropy(hs, w, labels, b, reduction=reduction)
+    got, = torch.autograd.grad(loss.sum(), hs)
+    assert torch.equal(got, want) and count["unpack"] == count["pack"] > 0
