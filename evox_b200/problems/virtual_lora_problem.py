@@ -99,9 +99,10 @@ class VirtualLoRAProblem(Problem):
     def _project(self, h: torch.Tensor, seeds: torch.Tensor, i: int) -> torch.Tensor:
         """h A^T (pop, batch, rank) of weight block `i` in fp32."""
         pop, batch, k = h.shape
+        h = h.to(torch.float32)
         a = philox_normal(seeds, self.lora_rank * k, self.counter_offsets[i]).view(pop, self.lora_rank, k)
         t = torch.empty(pop, batch, self.lora_rank, dtype=torch.float32, device=h.device)
-        _cabi.check(_cabi.lib.evox_lora_down(_cabi.ptr(h.to(torch.float32)), 0, _cabi.ptr(a), pop, batch, k, self.lora_rank, _cabi.ptr(t),
+        _cabi.check(_cabi.lib.evox_lora_down(_cabi.ptr(h), 0, _cabi.ptr(a), pop, batch, k, self.lora_rank, _cabi.ptr(t),
                                              _cabi.stream_ptr(h.device)))
         return t
 
