@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   }
 }
 
-// Tensors per launch: 2, 8 or 30 KB of arguments (32,764 bytes are the limit). A launch pays for copying what it carries: both
+// Tensors per launch, 20 bytes each: 2, 8 or 30 KB of arguments (32,764 bytes are the limit). A launch pays for copying what it carries: both
 // launches for 301 tensors take the host 18 us with 30 KB each, 11 with 8.
 constexpr int kSmall = 96, kMiddle = 400, kLarge = 1500;
 

@@ -21,10 +21,11 @@
 //
 // The product kernel is persistent, a CTA pair per 256 x 256 tile (cta_group::2): warp 0 feeds a six-stage ring
 // by TMA, one thread of the leader issues tcgen05.mma into one of two 256-column accumulators, eight warps
-// empty the other one. All waits are bounded; a wait that gives up sets the error flag and every role leaves.
+// empty the other one. All waits are bounded; a wait that gives up sets the status word and every role leaves. While the
+// word is set losses and gradients come out as NaN.
 //
 // Measured (bf16, device time): loss of 2,048 x 2,048 x 32,768 187 us = 1,470 TFLOP/s, of 16,384 x 4,096 x 131,072 13.4 ms =
-// 1,315 TFLOP/s under the power cap; with gradients 598 us and (8,192 rows) 20.8 ms. The tensor pipe is busy 78 % of the
+// 1,315 TFLOP/s under the power cap; with gradients 600 to 690 us and (8,192 rows) 20.8 to 21.8 ms. The tensor pipe is busy 78 % of the
 // logits product (its shared memory is: 64 KB of tiles written and as much read per 512 tensor cycles and SM) and
 // 94 % of the gradient products; the rescaling pass is 3 % (4,096 features) to 9 % (2,048) of a step.
 #include <cuda_bf16.h>
@@ -553,7 +554,9 @@ __global__ void __launch_bounds__(kThreads, 1) xent_product_kernel(const __grid_
 // nearly nothing but the weight (ten stages). Products into one accumulator follow one another at about 160 cycles
 // however narrow they are, so the four of a block go to four accumulators. Accumulator lanes are weight rows, so the softmax statistics of a token
 // run across lanes and the four warps that share a slice of 128. Measured: one token, 32,000 x 4,096: 54 us with the joining
-// kernel (4.9 TB/s of the weight; 60.7 us as a 256 x 256 tile with one row in use).
+// kernel (4.9 TB/s of the weight; 60.7 us as a 256 x 256 tile with one row in use). Two columns of 32 are what a stage's token
+// tile holds, hence 64 rows; at that many, here and as 256 x 256 tiles (loss / gradient, us): 4,096 x 32,000 58 / 170 and 63 / 174,
+// 2,048 x 131,072 102 / 328 and 116 / 329, 2,048 x 8,000 20 / 45 and 22 / 48, 256 x 1,000 10.3 / 23.1 and 10.5 / 21.5.
 // ---------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
 constexpr int kFewSums = BK / 16;       // accumulators at a time, one for each product of a block
