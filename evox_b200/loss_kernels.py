@@ -191,7 +191,9 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     start on 16-byte boundaries are copied); `labels` (...) int64; `bias` (vocab,). Rows labelled `ignore_index`
     have loss 0, do not count in the mean and get zero gradients, whatever they hold; a label
     outside the vocabulary gives NaN. `reduction`: "mean", "sum" or "none" (losses shaped like `labels`).
-    Differentiable once in `h`, `weight` and `bias`, in reverse mode (a forward-mode tangent is refused); the gradient holds 16-bit exponentials of `chunk_rows` rows at a time
+    Differentiable once in `h`, `weight` and `bias`, in reverse mode (a forward-mode tangent is refused). The softmax gradient
+    is rounded to the operands' type before its two products; a mean or sum of bf16 operands stores dh and dweight from the
+    forward pass on, elsewhere backward computes them. The gradient holds 16-bit exponentials of `chunk_rows` rows at a time
     (default: all, up to 2 GiB of them; a bias gradient doubles the bytes)."""
     _check_chunk(chunk_rows)
     _refuse_tangents(h, weight, bias)
